@@ -16,7 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libheartmula_b200.so"
 
 HM_SRC_F16, HM_SRC_RMS, HM_SRC_EMB = 0, 1, 2
 HM_EPI_STORE, HM_EPI_ROPE_KV, HM_EPI_SILU = 0, 1, 2
-HM_ERR_TIMEOUT, HM_ERR_BADINDEX = 1, 2
+HM_ERR_TIMEOUT, HM_ERR_BADINDEX, HM_ERR_NOPAGES = 1, 2, 4
 HM_EARG = -1
 HM_DT_F32, HM_DT_BF16, HM_DT_F16 = 0, 1, 2
 HM_ENOSPACE = -2
@@ -60,6 +60,18 @@ class ConvDesc(C.Structure):
                 ("bn", C.c_int)]
 
 
+class PageState(C.Structure):
+    """hm_page_state: tables, lengths and reference counts of a paged KV cache."""
+    _fields_ = [("table", _P), ("table_ld", _I64), ("lens", _P), ("refs", _P), ("err", _P),
+                ("n_seqs", C.c_int), ("max_pages", C.c_int), ("n_pages", C.c_int), ("page", C.c_int)]
+
+
+class PagePoolDesc(C.Structure):
+    """hm_page_pool: the K and V pages of every layer."""
+    _fields_ = [("k", _P), ("v", _P), ("layers", C.c_int), ("n_pages", C.c_int), ("Hk", C.c_int), ("page", C.c_int),
+                ("row_bytes", C.c_int)]
+
+
 SIGNATURES = {
     "hm_gemv_i8": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _P, _SZ, _P, _I, _P, _I, _I, _P]),
     "hm_gemv_i8_fused": (_I, [C.POINTER(GemvDesc), _P]),
@@ -82,6 +94,14 @@ SIGNATURES = {
     "hm_gemm_f16w": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P]),
     "hm_dequant_i8_f16": (_I, [_P, _P, _I64, _P]),
     "hm_prefill_attn": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P]),
+    "hm_pages_workspace_bytes": (_SZ, [_I, _I]),
+    "hm_pages_grow": (_I, [C.POINTER(PageState), _P, _I, _I, _P]),
+    "hm_pages_free": (_I, [C.POINTER(PageState), _P, _I, _P]),
+    "hm_pages_fork": (_I, [C.POINTER(PageState), C.POINTER(PagePoolDesc), _P, _P, _I, _P, _SZ, _P]),
+    "hm_pages_copy": (_I, [C.POINTER(PagePoolDesc), _P, _P, _I, _P, _SZ, _P, _P]),
+    "hm_pages_compact": (_I, [C.POINTER(PageState), C.POINTER(PagePoolDesc), _P, _P, _SZ, _P]),
+    "hm_rope_pages": (_I, [_P, _I64, _P, _I, _P, _P, _I64, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+                           _P, _P]),
     "hm_conv1d_gemm": (_I, [C.POINTER(ConvDesc), _P]),
     "hm_codec_attn": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I64, _I64, _F, _P, _P]),
     "hm_codec_norm_mod": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _F, _I, _P]),
@@ -171,5 +191,6 @@ def abi_mismatches() -> list[str]:
     L = lib()
     want = {0: C.sizeof(RowSrc), 1: C.sizeof(GemvDesc), 2: GemvDesc.src.offset, 3: GemvDesc.ws.offset,
             4: GemvDesc.pdl.offset, 5: GemvDesc.l2_keep.offset, 6: C.sizeof(ConvDesc), 7: ConvDesc.B.offset,
-            8: ConvDesc.scale.offset, 9: ConvDesc.bn.offset}
+            8: ConvDesc.scale.offset, 9: ConvDesc.bn.offset, 10: C.sizeof(PageState), 11: PageState.page.offset,
+            12: C.sizeof(PagePoolDesc), 13: PagePoolDesc.row_bytes.offset}
     return [f"layout[{k}]: C {L.hm_abi_layout(k)} vs ctypes {v}" for k, v in want.items() if L.hm_abi_layout(k) != v]

@@ -1245,6 +1245,10 @@ extern "C" size_t hm_abi_layout(int which) {
     case 7: return offsetof(hm_conv_desc, B);
     case 8: return offsetof(hm_conv_desc, scale);
     case 9: return offsetof(hm_conv_desc, bn);
+    case 10: return sizeof(hm_page_state);
+    case 11: return offsetof(hm_page_state, page);
+    case 12: return sizeof(hm_page_pool);
+    case 13: return offsetof(hm_page_pool, row_bytes);
     default: return 0;
   }
 }

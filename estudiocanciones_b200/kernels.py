@@ -251,6 +251,211 @@ def prefill_attn(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, P: int, o:
     return o
 
 
+# ----------------------------------------------------------------------------- call plumbing
+# The calls below take a few microseconds on the GPU, so their host side is kept short: messages
+# are built only when a check fails, the stream is read as a raw handle, and the device is
+# switched only when the tensors lie on another one than the current.
+_DT = {torch.float16: _lib.HM_DT_F16, torch.bfloat16: _lib.HM_DT_BF16}
+_ERR_PTRS: dict[int, int] = {}
+
+
+def _device_of(what: str, *ts) -> int:
+    """The index of the CUDA device that all of ``ts`` (None: absent) lie on."""
+    idx = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != idx or idx < 0):
+            _need_cuda(*ts)
+            raise HMError(f"{what}: the tensors lie on different devices")
+    return idx
+
+
+def _err_ptr(idx: int) -> int:
+    p = _ERR_PTRS.get(idx)
+    if p is None:
+        p = _ERR_PTRS[idx] = error_word(torch.device("cuda", idx)).data_ptr()
+    return p
+
+
+def _launch(idx: int, what: str, *args) -> None:
+    """The entry point ``what`` with ``args`` on the current stream of device ``idx``."""
+    fn = getattr(_lib.lib(), what)
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        check(rc, what)
+
+
+# ----------------------------------------------------------------------------- pages of a KV cache
+MAX_LIST = 1024   # sequences or pages of one call
+
+
+def _ids(what: str, ids, like) -> torch.Tensor:
+    """A call's list: an int32 tensor on ``like``'s device, or a sequence of ints (copied there)."""
+    if not torch.is_tensor(ids):
+        if torch.cuda.is_current_stream_capturing():
+            raise HMError(f"{what}: pass lists as device tensors inside a capture")
+        ids = torch.tensor(list(ids), dtype=torch.int32, device=like.device)
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.get_device() != like.get_device():
+        raise HMError(f"{what}: lists are contiguous int32 vectors on the cache's device")
+    if not 1 <= ids.numel() <= MAX_LIST:
+        raise HMError(f"{what}: a list holds 1 to {MAX_LIST} entries")
+    return ids
+
+
+def _is_table(t) -> bool:
+    return (t.dtype == torch.int32 and t.dim() == 2 and t.numel() > 0 and t.stride(1) == 1 and
+            t.stride(0) >= t.shape[1])
+
+
+def _page_state(what: str, table, lens, refs, page: int):
+    """(device index, hm_page_state).  ``lens`` None: a call that does not read it."""
+    idx = _device_of(what, table, lens, refs)
+    if not _is_table(table):
+        raise HMError(f"{what}: table is int32 [sequences, pages], rows contiguous")
+    n, mp = table.shape
+    if lens is not None and (lens.dtype != torch.int64 or lens.dim() != 1 or lens.numel() != n or
+                             not lens.is_contiguous()):
+        raise HMError(f"{what}: lens is int64 [sequences]")
+    if refs.dtype != torch.int32 or refs.dim() != 1 or refs.numel() < 1 or not refs.is_contiguous():
+        raise HMError(f"{what}: refs is int32 [pages of the pool]")
+    if not 1 <= page <= 1024:
+        raise HMError(f"{what}: a page holds 1 to 1024 positions")
+    return idx, _lib.PageState(table.data_ptr(), table.stride(0), None if lens is None else lens.data_ptr(),
+                               refs.data_ptr(), _err_ptr(idx), n, mp, refs.numel(), page)
+
+
+def _page_pool(what: str, k, v):
+    if (k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous() or
+            k.numel() == 0):
+        raise HMError(f"{what}: k and v are contiguous [layers, pages, Hk, page, hd] of one type")
+    layers, n_pages, hk, page, hd = k.shape
+    row = hd * k.element_size()
+    if row % 16:
+        raise HMError(f"{what}: a position of a head is a multiple of 16 bytes")
+    return _lib.PagePoolDesc(k.data_ptr(), v.data_ptr(), layers, n_pages, hk, page, row)
+
+
+def pages_grow(table, lens, refs, page: int, seqs, n: int = 1) -> None:
+    """Room for ``n`` more positions of every sequence in ``seqs``: pages are taken from the free
+    ones (``refs == 0``), lowest number first, and ``lens`` grows by ``n``.
+
+    This and the other ``pages_*`` calls are decided on the device, so they can be captured: a
+    call with a bad list, or more pages than are free, changes nothing and sets
+    ``HM_ERR_BADINDEX`` / ``HM_ERR_NOPAGES`` in the device's error word (:func:`read_errors`).
+    Lists hold sequence (page) numbers, at most 1024; a negative entry is skipped."""
+    idx, st = _page_state("pages_grow", table, lens, refs, page)
+    seqs = _ids("pages_grow", seqs, table)
+    if not 0 <= n < 1 << 31:
+        raise HMError("pages_grow: n >= 0 positions")
+    _launch(idx, "hm_pages_grow", st, seqs.data_ptr(), seqs.numel(), n)
+
+
+def pages_free(table, lens, refs, seqs) -> None:
+    """The sequences in ``seqs`` end: their pages lose a holder, their rows become -1."""
+    idx, st = _page_state("pages_free", table, lens, refs, 1)
+    seqs = _ids("pages_free", seqs, table)
+    _launch(idx, "hm_pages_free", st, seqs.data_ptr(), seqs.numel())
+
+
+def _moves(what: str, n_moves: int, n_pages: int, like):
+    """Scratch of a call that moves pages: (tensor, bytes)."""
+    nbytes = _lib.lib().hm_pages_workspace_bytes(n_moves, n_pages)
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes
+
+
+def pages_fork(k, v, table, lens, refs, src, dst) -> None:
+    """Empty sequence ``dst[i]`` becomes a copy of sequence ``src[i]``: full pages are shared, the
+    positions of a partial last page are copied (every layer, K and V) into a free page."""
+    _device_of("pages_fork", table, k, v)
+    pool = _page_pool("pages_fork", k, v)
+    idx, st = _page_state("pages_fork", table, lens, refs, pool.page)
+    if refs.numel() != pool.n_pages:
+        raise HMError("pages_fork: refs has one count per page of the pool")
+    src, dst = _ids("pages_fork", src, table), _ids("pages_fork", dst, table)
+    n = dst.numel()
+    if src.numel() != n:
+        raise HMError("pages_fork: src and dst have the same length")
+    ws, nbytes = _moves("pages_fork", n, 0, table)
+    _launch(idx, "hm_pages_fork", st, pool, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), nbytes)
+
+
+def pages_copy(k, v, src, dst) -> None:
+    """Pages ``dst[i]`` become copies of pages ``src[i]`` in every layer, K and V.  No page may be a
+    target twice, or a target and a source."""
+    idx = _device_of("pages_copy", k, v)
+    pool = _page_pool("pages_copy", k, v)
+    src, dst = _ids("pages_copy", src, k), _ids("pages_copy", dst, k)
+    n = dst.numel()
+    if src.numel() != n:
+        raise HMError("pages_copy: src and dst have the same length")
+    ws, nbytes = _moves("pages_copy", n, 0, k)
+    _launch(idx, "hm_pages_copy", pool, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), nbytes, _err_ptr(idx))
+
+
+def pages_compact(k, v, table, refs) -> torch.Tensor:
+    """Pack the live pages (``refs > 0``) into the lowest numbers: those at or above their count
+    move into the free ones below it, in ascending order, and the table follows.  Returns the
+    count, int32 ``[1]`` on the device."""
+    _device_of("pages_compact", table, k, v)
+    pool = _page_pool("pages_compact", k, v)
+    idx, st = _page_state("pages_compact", table, None, refs, pool.page)
+    if refs.numel() != pool.n_pages:
+        raise HMError("pages_compact: refs has one count per page of the pool")
+    n_live = torch.empty(1, dtype=torch.int32, device=table.device)
+    ws, nbytes = _moves("pages_compact", pool.n_pages // 2, pool.n_pages, table)
+    _launch(idx, "hm_pages_compact", st, pool, n_live.data_ptr(), ws.data_ptr(), nbytes)
+    return n_live
+
+
+def _layer_pages(what: str, k, v, table, seqs, R: int, S: int) -> None:
+    """One layer's pool and the rows of its table that R query rows use."""
+    if (k.dtype not in _DT or k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or
+            not v.is_contiguous() or k.numel() == 0):
+        raise HMError(f"{what}: k and v are contiguous fp16 or bf16 [pages, Hk, page, hd]")
+    if not _is_table(table):
+        raise HMError(f"{what}: table is int32 [sequences, pages], rows contiguous")
+    if S < 1 or R < 1 or R % S:
+        raise HMError(f"{what}: S >= 1 rows of every sequence")
+    if seqs is None:
+        if R // S > table.shape[0]:
+            raise HMError(f"{what}: the table has a row for every sequence")
+    elif seqs.dtype != torch.int32 or seqs.shape != (R // S,) or not seqs.is_contiguous():
+        raise HMError(f"{what}: seqs is int32 [sequences]")
+
+
+def _is_rows(t, R: int, W: int) -> bool:
+    """[R, W] with contiguous rows."""
+    return t.dim() == 2 and t.shape[0] == R and t.shape[1] == W and t.stride(1) == 1
+
+
+def rope_pages(qkv, rope, pos, q_out, k, v, table, S: int, Hq: int, Hk: int, seqs=None) -> None:
+    """:func:`rope_cache` into pages: RoPE of q and k at ``pos[r]``, k and v written into the page
+    that row ``r // S`` of the table (``seqs[r // S]`` when given) holds for that position.
+    A padding row has ``pos[r] < 0``: its ``q_out`` is zero and nothing is written."""
+    idx = _device_of("rope_pages", qkv, rope, pos, q_out, k, v, table, seqs)
+    R = qkv.shape[0]
+    _layer_pages("rope_pages", k, v, table, seqs, R, S)
+    n_pages, hk, page, hd = k.shape
+    if hk != Hk or hd % 8:
+        raise HMError("rope_pages: Hk heads of a multiple of 8 dims")
+    if qkv.dtype != k.dtype or q_out.dtype != k.dtype or not _is_rows(qkv, R, (Hq + 2 * Hk) * hd):
+        raise HMError("rope_pages: qkv [R, (Hq + 2 Hk) * hd] of the cache's type")
+    if not _is_rows(q_out, R, Hq * hd):
+        raise HMError("rope_pages: q_out [R, Hq * hd]")
+    if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.shape[1:] != (hd // 2, 2):
+        raise HMError("rope_pages: rope is float32 [positions, hd / 2, 2]")
+    if pos.dtype != torch.int64 or pos.shape != (R,) or not pos.is_contiguous():
+        raise HMError("rope_pages: pos is int64 [R]")
+    _launch(idx, "hm_rope_pages", qkv.data_ptr(), qkv.stride(0) if R > 1 else qkv.shape[1], rope.data_ptr(),
+            rope.shape[0], pos.data_ptr(), q_out.data_ptr(), q_out.stride(0) if R > 1 else q_out.shape[1],
+            k.data_ptr(), v.data_ptr(), _DT[k.dtype], table.data_ptr(), table.stride(0),
+            None if seqs is None else seqs.data_ptr(), table.shape[0], table.shape[1], n_pages, page, R, S, Hq, Hk, hd,
+            _err_ptr(idx))
+
+
 # ----------------------------------------------------------------------------- raw-launch stand-ins
 class _Launch:
     """A kernel name that launches with the reference's ``kernel[grid](*args, **meta)``

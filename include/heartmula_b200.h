@@ -41,6 +41,7 @@ typedef struct CUstream_st* hm_stream_t; /* == cudaStream_t */
 /* device error-word bits */
 #define HM_ERR_TIMEOUT 1   /* a bounded wait gave up */
 #define HM_ERR_BADINDEX 2  /* token id / position outside its table; access skipped */
+#define HM_ERR_NOPAGES 4   /* a page pool has too few free pages for a call; the call changed nothing */
 
 /* ------------------------------------------------------------------ int8 GEMV
  * y[m, n] = fp16( sum_k x[m,k] * w[n,k] * s[n] ) (+ res[m, n] in fp16),  M <= 32, K % 16 == 0.
@@ -245,6 +246,63 @@ int hm_dequant_i8_f16(const int8_t* w, void* out, int64_t n, hm_stream_t stream)
 int hm_prefill_attn(const void* q, const void* kc, const void* vc, void* o, int B, int P, int Hq, int Hk, int hd,
                     int L, float scale, int* err, hm_stream_t stream);
 
+/* ------------------------------------------------------------------ pages of a KV cache
+ * No counterpart in the reference, whose static cache (app/engine.py:119-121) holds the prompt
+ * once per row.  K and V lie in pools [layers, n_pages, Hk, page, hd]; sequence s holds
+ * lens[s] positions in the pages table[s*table_ld + 0 ..] (-1 = none), refs[p] sequences hold
+ * page p (0 = free).  All of this is device memory, and every call below is decided on the
+ * device: it checks its whole list first and either applies all of it or sets a bit in `err`
+ * and changes nothing (HM_ERR_BADINDEX: a bad or repeated entry, or a table that disagrees
+ * with refs; HM_ERR_NOPAGES: too few free pages).  Free pages are handed out lowest number
+ * first, in the order of the list.  Lists hold 1 to 1024 int32 entries; a negative entry (of
+ * dst, for a pair) is skipped.  Calls on one state must not overlap on the GPU. */
+typedef struct {
+  int* table;
+  int64_t table_ld;
+  int64_t* lens;                /* hm_pages_compact does not use it (NULL) */
+  int* refs;
+  int* err;
+  int n_seqs, max_pages, n_pages, page;
+} hm_page_state;
+
+typedef struct {
+  void* k;
+  void* v;
+  int layers, n_pages, Hk, page;
+  int row_bytes;                /* hd * element size, a multiple of 16 */
+} hm_page_pool;
+
+/* Scratch of the calls that move data: hm_pages_fork and hm_pages_copy (n_moves = n, n_pages = 0),
+ * hm_pages_compact (n_moves = n_pages / 2, n_pages). */
+size_t hm_pages_workspace_bytes(int n_moves, int n_pages);
+/* Room for `add` more positions of every listed sequence: takes pages, lens += add.  A partial
+ * last page must be held by its sequence alone (hm_pages_fork never shares one). */
+int hm_pages_grow(const hm_page_state* s, const int* seqs, int n, int add, hm_stream_t stream);
+/* The listed sequences end: their pages lose a holder, their rows become -1, lens = 0. */
+int hm_pages_free(const hm_page_state* s, const int* seqs, int n, hm_stream_t stream);
+/* Sequence dst[i] (empty) becomes a copy of src[i]: full pages are shared, the positions of a
+ * partial last page are copied into a free page in every layer.  A source may be listed
+ * several times; no target may be listed twice or be a source. */
+int hm_pages_fork(const hm_page_state* s, const hm_page_pool* pool, const int* src, const int* dst, int n, void* ws,
+                  size_t ws_bytes, hm_stream_t stream);
+/* Pages dst[i] <- src[i] in every layer, K and V.  No target may be listed twice or be a source. */
+int hm_pages_copy(const hm_page_pool* pool, const int* src, const int* dst, int n, void* ws, size_t ws_bytes, int* err,
+                  hm_stream_t stream);
+/* Live pages at or above *n_live (their number, written) move into the free ones below it, i-th
+ * to i-th in ascending order, and the table follows: afterwards pages [0, *n_live) are live. */
+int hm_pages_compact(const hm_page_state* s, const hm_page_pool* pool, int* n_live, void* ws, size_t ws_bytes,
+                     hm_stream_t stream);
+
+/* hm_rope_kv_write into pages (app/kernels.py:79-107 with a page table): row r of qkv
+ * [R, (Hq+2Hk)*hd] (row pitch ld_qkv) belongs to table row seqs[r / S] (seqs NULL: r / S) at
+ * position pos[r]; q_out [R, Hq*hd] (pitch ld_q), k / v one layer's pool [n_pages, Hk, page, hd].
+ * dtype HM_DT_F16 or HM_DT_BF16 (qkv, q_out, k, v).  pos[r] < 0: a padding row, q_out zero and
+ * nothing written; a position without a page: the same, with HM_ERR_BADINDEX. */
+int hm_rope_pages(const void* qkv, int64_t ld_qkv, const float* rope, int rope_rows, const int64_t* pos, void* q_out,
+                  int64_t ld_q, void* k, void* v, int dtype, const int* table, int64_t table_ld, const int* seqs,
+                  int n_table, int max_pages, int n_pages, int page, int R, int S, int Hq, int Hk, int hd, int* err,
+                  hm_stream_t stream);
+
 /* ------------------------------------------------------------------ HeartCodec detokenize
  * The codec turns the [8, T] token streams into audio (app/codec_lite.py:63-75 ->
  * HeartCodec.detokenize, app/heartcodec/modeling_heartcodec.py:57-204): a flow-matching
@@ -356,7 +414,8 @@ int hm_decode_attn_box_form(const void* cache, int64_t rows);
  * 0 sizeof(hm_row_src), 1 sizeof(hm_gemv_desc), 2 offsetof(hm_gemv_desc, src),
  * 3 offsetof(hm_gemv_desc, ws), 4 offsetof(hm_gemv_desc, pdl), 5 offsetof(hm_gemv_desc, l2_keep),
  * 6 sizeof(hm_conv_desc), 7 offsetof(hm_conv_desc, B), 8 offsetof(hm_conv_desc, scale),
- * 9 offsetof(hm_conv_desc, bn). */
+ * 9 offsetof(hm_conv_desc, bn), 10 sizeof(hm_page_state), 11 offsetof(hm_page_state, page),
+ * 12 sizeof(hm_page_pool), 13 offsetof(hm_page_pool, row_bytes). */
 size_t hm_abi_layout(int which);
 const char* hm_version(void);
 

@@ -72,6 +72,16 @@ class PagePoolDesc(C.Structure):
                 ("row_bytes", C.c_int)]
 
 
+class PrefixAttnDesc(C.Structure):
+    """hm_prefix_attn_desc: decode attention over a paged cache with shared prefixes."""
+    _fields_ = [("q", _P), ("ld_q", _I64), ("o", _P), ("ld_o", _I64), ("k", _P), ("v", _P), ("pos", _P),
+                ("table", _P), ("table_ld", _I64), ("seqs", _P), ("gstart", _P), ("owner", _P), ("plen", _P),
+                ("ws", _P), ("ws_bytes", C.c_size_t), ("err", _P),
+                ("dtype", C.c_int), ("R", C.c_int), ("S", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("hd", C.c_int),
+                ("n_table", C.c_int), ("max_pages", C.c_int), ("n_pages", C.c_int), ("page", C.c_int),
+                ("n_groups", C.c_int), ("scale", C.c_float)]
+
+
 SIGNATURES = {
     "hm_gemv_i8": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _P, _SZ, _P, _I, _P, _I, _I, _P]),
     "hm_gemv_i8_fused": (_I, [C.POINTER(GemvDesc), _P]),
@@ -94,6 +104,8 @@ SIGNATURES = {
     "hm_gemm_f16w": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P]),
     "hm_dequant_i8_f16": (_I, [_P, _P, _I64, _P]),
     "hm_prefill_attn": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P]),
+    "hm_prefix_attn": (_I, [C.POINTER(PrefixAttnDesc), _P]),
+    "hm_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "hm_pages_workspace_bytes": (_SZ, [_I, _I]),
     "hm_pages_grow": (_I, [C.POINTER(PageState), _P, _I, _I, _P]),
     "hm_pages_free": (_I, [C.POINTER(PageState), _P, _I, _P]),
@@ -192,5 +204,6 @@ def abi_mismatches() -> list[str]:
     want = {0: C.sizeof(RowSrc), 1: C.sizeof(GemvDesc), 2: GemvDesc.src.offset, 3: GemvDesc.ws.offset,
             4: GemvDesc.pdl.offset, 5: GemvDesc.l2_keep.offset, 6: C.sizeof(ConvDesc), 7: ConvDesc.B.offset,
             8: ConvDesc.scale.offset, 9: ConvDesc.bn.offset, 10: C.sizeof(PageState), 11: PageState.page.offset,
-            12: C.sizeof(PagePoolDesc), 13: PagePoolDesc.row_bytes.offset}
+            12: C.sizeof(PagePoolDesc), 13: PagePoolDesc.row_bytes.offset,
+            14: C.sizeof(PrefixAttnDesc), 15: PrefixAttnDesc.scale.offset}
     return [f"layout[{k}]: C {L.hm_abi_layout(k)} vs ctypes {v}" for k, v in want.items() if L.hm_abi_layout(k) != v]

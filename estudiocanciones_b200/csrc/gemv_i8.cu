@@ -1249,6 +1249,8 @@ extern "C" size_t hm_abi_layout(int which) {
     case 11: return offsetof(hm_page_state, page);
     case 12: return sizeof(hm_page_pool);
     case 13: return offsetof(hm_page_pool, row_bytes);
+    case 14: return sizeof(hm_prefix_attn_desc);
+    case 15: return offsetof(hm_prefix_attn_desc, scale);
     default: return 0;
   }
 }

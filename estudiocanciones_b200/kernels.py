@@ -456,6 +456,67 @@ def rope_pages(qkv, rope, pos, q_out, k, v, table, S: int, Hq: int, Hk: int, seq
             _err_ptr(idx))
 
 
+_SMS: dict[int, int] = {}
+
+
+def _sms(idx: int) -> int:
+    n = _SMS.get(idx)
+    if n is None:
+        n = _SMS[idx] = torch.cuda.get_device_properties(idx).multi_processor_count
+    return n
+
+
+def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int = 1, o=None, scale=None,
+                seqs=None) -> torch.Tensor:
+    """Decode attention over pages, the prefix that a group of sequences shares read once for all.
+
+    Row r of ``q [R, Hq * hd]`` belongs to sequence ``b = r // S``, whose pages stand in row ``b`` of
+    ``table`` (``seqs[b]`` when given), and attends to positions ``[0, pos[r]]`` of one layer's pool
+    ``k, v [pages, Hk, page, hd]`` (fp16 or bf16; hd 64, 128, 256; page 16, 32 or a multiple of 64).
+    Sequences ``gstart[g] <= b < gstart[g + 1]`` hold the same K and V at positions
+    ``[0, plen[g])``, read through table row ``owner[g]`` (``gstart [groups + 1]``, ``owner`` and ``plen
+    [groups]`` int32 on the device, so a captured call serves every frame); without groups every
+    sequence reads its own pages.  ``pos[r] < 0`` is a padding row and gives zeros.  Returns ``o``
+    like ``q``."""
+    idx = _device_of("prefix_attn", q, k, v, table, pos, gstart, owner, plen, o, seqs)
+    if q.dim() != 2:
+        raise HMError("prefix_attn: q [R, Hq * hd]")
+    R, W = q.shape
+    _layer_pages("prefix_attn", k, v, table, seqs, R, S)
+    n_pages, Hk, page, hd = k.shape
+    Hq = W // hd
+    if q.dtype != k.dtype or W != Hq * hd or Hq < Hk or Hq % Hk or q.stride(1) != 1:
+        raise HMError("prefix_attn: q [R, Hq * hd] of the cache's type, Hq a multiple of Hk")
+    if o is None:
+        o = torch.empty(R, W, dtype=q.dtype, device=q.device)
+    elif o.dtype != q.dtype or not _is_rows(o, R, W):
+        raise HMError("prefix_attn: o is like q")
+    if pos.dtype != torch.int64 or pos.dim() != 1 or pos.numel() != R or not pos.is_contiguous():
+        raise HMError("prefix_attn: pos is int64 [R]")
+    groups = 0
+    if gstart is not None:
+        groups = gstart.numel() - 1
+        if owner is None or plen is None:
+            raise HMError("prefix_attn: gstart comes with owner and plen")
+        for t, n in ((gstart, groups + 1), (owner, groups), (plen, groups)):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or n < 0 or not t.is_contiguous():
+                raise HMError("prefix_attn: gstart [groups + 1], owner and plen [groups] are int32 vectors")
+    elif owner is not None or plen is not None:
+        raise HMError("prefix_attn: owner and plen come with gstart")
+    nbytes = _lib.lib().hm_prefix_attn_workspace_bytes(R, S, Hq, Hk, hd, groups, _sms(idx))
+    if nbytes == 0:
+        raise HMError("prefix_attn: hd 64, 128 or 256, up to 64 query heads per KV head and 1024 row blocks")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    d = _lib.PrefixAttnDesc(q.data_ptr(), q.stride(0) if R > 1 else W, o.data_ptr(), o.stride(0) if R > 1 else W,
+                            k.data_ptr(), v.data_ptr(), pos.data_ptr(), table.data_ptr(), table.stride(0),
+                            None if seqs is None else seqs.data_ptr(), gstart.data_ptr() if groups > 0 else None,
+                            owner.data_ptr() if groups > 0 else None, plen.data_ptr() if groups > 0 else None,
+                            ws.data_ptr(), nbytes, _err_ptr(idx), _DT[k.dtype], R, S, Hq, Hk, hd, table.shape[0],
+                            table.shape[1], n_pages, page, groups, 1.0 / math.sqrt(hd) if scale is None else scale)
+    _launch(idx, "hm_prefix_attn", d)
+    return o
+
+
 # ----------------------------------------------------------------------------- raw-launch stand-ins
 class _Launch:
     """A kernel name that launches with the reference's ``kernel[grid](*args, **meta)``

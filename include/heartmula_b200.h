@@ -207,6 +207,42 @@ size_t hm_decode_attn_workspace_bytes(int R, int Hq, int hd, int nsplit);
 int hm_decode_attn_noalloc(const void* q, const void* kc, const void* vc, const int64_t* pos, void* o, int R, int S,
                            int Hq, int Hk, int hd, int L, float scale, int nsplit, int* err, hm_stream_t stream);
 
+/* Decode attention over a paged cache for sequences that share a prefix (no counterpart in the
+ * reference, which reads every row's own copy of the prompt, app/kernels.py:112-167).
+ * Row r of q [R, Hq*hd] (pitch ld_q, R % S == 0) belongs to sequence b = r / S, whose pages stand
+ * in table row seqs[b] (seqs NULL: b), and attends to positions [0, pos[r]] of it; o like q.
+ * Sequences gstart[g] .. gstart[g+1] - 1 (gstart: n_groups + 1 ascending values) form group g and
+ * hold the same K and V at positions [0, plen[g]): those are read once, through table row
+ * owner[g].  Sequences outside every group (n_groups may be 0) read all their own pages.
+ * pos[r] < 0: a padding row, o = 0.  A bad position, table row, page or group entry sets
+ * HM_ERR_BADINDEX; positions without a page, and rows with a bad position, are left out.
+ * hd 64, 128 or 256; page 16, 32 or a multiple of 64; Hq / Hk <= 64; dtype HM_DT_F16 or
+ * HM_DT_BF16 (q, k, v, o); at most 1024 row blocks: R*G/64 + n_groups + R/S * ceil(S*G / 64).
+ * ws: hm_prefix_attn_workspace_bytes(..., sms = hm_device_sm_count), 16-byte aligned, not shared by calls that
+ * overlap on the GPU. */
+typedef struct {
+  const void* q;
+  int64_t ld_q;
+  void* o;
+  int64_t ld_o;
+  const void* k;                /* one layer's pool [n_pages, Hk, page, hd] */
+  const void* v;
+  const int64_t* pos;
+  const int* table;
+  int64_t table_ld;
+  const int* seqs;
+  const int* gstart;
+  const int* owner;
+  const int* plen;
+  void* ws;
+  size_t ws_bytes;
+  int* err;
+  int dtype, R, S, Hq, Hk, hd, n_table, max_pages, n_pages, page, n_groups;
+  float scale;
+} hm_prefix_attn_desc;
+int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream);
+size_t hm_prefix_attn_workspace_bytes(int R, int S, int Hq, int Hk, int hd, int n_groups, int sms);
+
 /* ------------------------------------------------------------------ sampler
  * _guided + _sample (app/engine.py:291-305) for one codebook: optional CFG mix
  * (rows [0,N) conditional, [N,2N) unconditional, fp16 arithmetic), /temp,
@@ -415,7 +451,8 @@ int hm_decode_attn_box_form(const void* cache, int64_t rows);
  * 3 offsetof(hm_gemv_desc, ws), 4 offsetof(hm_gemv_desc, pdl), 5 offsetof(hm_gemv_desc, l2_keep),
  * 6 sizeof(hm_conv_desc), 7 offsetof(hm_conv_desc, B), 8 offsetof(hm_conv_desc, scale),
  * 9 offsetof(hm_conv_desc, bn), 10 sizeof(hm_page_state), 11 offsetof(hm_page_state, page),
- * 12 sizeof(hm_page_pool), 13 offsetof(hm_page_pool, row_bytes). */
+ * 12 sizeof(hm_page_pool), 13 offsetof(hm_page_pool, row_bytes), 14 sizeof(hm_prefix_attn_desc),
+ * 15 offsetof(hm_prefix_attn_desc, scale). */
 size_t hm_abi_layout(int which);
 const char* hm_version(void);
 

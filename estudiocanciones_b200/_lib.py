@@ -104,6 +104,10 @@ SIGNATURES = {
     "hm_gemm_f16w": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P]),
     "hm_dequant_i8_f16": (_I, [_P, _P, _I64, _P]),
     "hm_prefill_attn": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P]),
+    "hm_quant_tokens": (_I, [_P, _I64, _I, _I, _I, _P, _I64, _P, _P]),
+    "hm_gemm_i8a8": (_I, [_P, _I64, _P, _I, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P]),
+    "hm_int8_mm_a8": (_I, [_P, _I64, _I, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _SZ, _P, _P]),
+    "hm_int8_mm_a8_workspace_bytes": (_SZ, [_I, _I]),
     "hm_prefix_attn": (_I, [C.POINTER(PrefixAttnDesc), _P]),
     "hm_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "hm_pages_workspace_bytes": (_SZ, [_I, _I]),

@@ -1,0 +1,728 @@
+// Matrix product in 8-bit integers with a scale for each token and each output channel (sm_100a).
+//
+//   q[m, k] = round(127 x[m, k] / amax[m]),  sx[m] = amax[m] / 127,  amax[m] = max_k |x[m, k]|
+//   acc[m, n] = sum_k q[m, k] * w[n, k]                              (int32, exact: K <= 131072)
+//   STORE: c[m, n] = acc * sx[m] * s[n]  (+ res[m, n])
+//   SILU : w = [w1; w3], c[m, f] = silu(a) * b,  a, b = the two halves' scaled sums
+// Everything after the integers is fp32 and rounded once to the activations' type (fp16, bf16).
+// The reference multiplies int8 weights with fp16 activations (app/kernels.py:20-54); with both
+// operands in 8 bits the tensor cores run twice as fast and the activations take half the bytes.
+//
+// quant_kernel: one CTA per token; the row stays in registers between the maximum and the
+// rounding, so x is read once (HBM: 3 bytes an element).  127 x is exact in fp32 (at most 18
+// bits), so one IEEE division decides the rounding; it is only taken where the product with the
+// reciprocal lies within 2^-15 of a half (its error is below 127 * 2^-23), else the cheap product
+// gives the same integer.
+//
+// Two products, both tcgen05.mma kind::i8 (K = 32 a step) fed by TMA (128-byte swizzle, K blocks of
+// 128 bytes) with the int32 sums in TMEM:
+//  * gemm_small: one 128 x BN tile per CTA, BN = 16 .. 128.  For few tokens the weights are all the
+//    traffic, so BN is chosen to put the weight stream on as many SMs as there are, and a CTA
+//    keeps a ring of up to ~100 KB in flight.  Only the rows that exist are loaded: the MMA's
+//    other rows read whatever lies behind them in shared memory, and nobody reads their sums.
+//    In hm_int8_mm_a8 the weight stream starts before the quantisation has finished
+//    (programmatic dependent launch; the weights do not depend on it).
+//  * gemm_pair: persistent 256 x 256 tiles on SM pairs (cta_group::2), two accumulators per CTA so
+//    that a tile's epilogue overlaps the next tile's products (the layout of gemm_f16w with twice
+//    the depth per byte).
+// The integer sums do not depend on the order, so both give the same result bit for bit.
+#include <cuda_bf16.h>
+
+#include <atomic>
+
+#include "hm_common.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+// ---------------------------------------------------------------- types
+template <typename T>
+struct Ty;
+template <>
+struct Ty<__half> {
+  static constexpr uint32_t kInf = 0x7c00u;
+  static HM_DEV float2 f2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static HM_DEV uint32_t pack(float a, float b) { return pack_h2(a, b); }
+  static HM_DEV float f(__half v) { return __half2float(v); }
+  static HM_DEV __half one(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Ty<__nv_bfloat16> {
+  static constexpr uint32_t kInf = 0x7f80u;
+  static HM_DEV float2 f2(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
+  static HM_DEV uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static HM_DEV float f(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static HM_DEV __nv_bfloat16 one(float v) { return __float2bfloat16_rn(v); }
+};
+
+// ---------------------------------------------------------------- quantisation of the tokens
+constexpr int kQThreads = 256;
+constexpr int kQChunks = 8;  // 8-element chunks a thread keeps in registers (K <= 16384)
+
+HM_DEV int quant1(float x, float inv, float amax) {
+  const float t = x * inv;
+  float r = rintf(t);
+  // near a half (or an overflowing reciprocal): the exact quotient decides
+  if (!(fabsf(t - r) < 0.5f - 3.0517578125e-5f)) r = rintf(__fdiv_rn(x * 127.f, amax));
+  return static_cast<int>(r);
+}
+
+template <typename T>
+HM_DEV uint2 quant8(uint4 v, float inv, float amax) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  uint32_t out[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float2 a = Ty<T>::f2(u[2 * h]), b = Ty<T>::f2(u[2 * h + 1]);
+    out[h] = (quant1(a.x, inv, amax) & 0xff) | ((quant1(a.y, inv, amax) & 0xff) << 8) |
+             ((quant1(b.x, inv, amax) & 0xff) << 16) | (static_cast<uint32_t>(quant1(b.y, inv, amax)) << 24);
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+// The largest |x| of 8 elements as 16-bit patterns (ordered like the values; inf and NaN on top).
+HM_DEV uint32_t top_bits(uint4 v, uint32_t top) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, u[i] & 0x7fff7fffu);
+  return top;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQThreads) quant_kernel(const T* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
+                                                          int64_t ldq, float* __restrict__ sx) {
+  __shared__ uint32_t red[kQThreads / 32];
+  pdl_trigger();
+  const int tid = threadIdx.x, nc = K / 8;
+  const uint4* row = reinterpret_cast<const uint4*>(x + blockIdx.x * ldx);
+  uint2* out = reinterpret_cast<uint2*>(q + blockIdx.x * ldq);
+  uint4 v[kQChunks];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) {
+    const int c = tid + i * kQThreads;
+    v[i] = c < nc ? row[c] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) top = top_bits(v[i], top);
+  for (int c = tid + kQChunks * kQThreads; c < nc; c += kQThreads) top = top_bits(row[c], top);
+  top = max(top & 0xffffu, top >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQThreads / 32; ++w) top = max(top, red[w]);
+  const float amax = Ty<T>::f2(top).x;
+  const bool zero = top == 0, bad = top >= Ty<T>::kInf;
+  const float inv = __fdiv_rn(127.f, amax);
+  // a row with an infinity or NaN has the scale NaN: its outputs are NaN, the other rows' are not
+  if (tid == 0) sx[blockIdx.x] = bad ? __int_as_float(0x7fffffff) : __fdiv_rn(amax, 127.f);
+  const bool none = zero || bad;
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) {
+    const int c = tid + i * kQThreads;
+    if (c < nc) out[c] = none ? make_uint2(0, 0) : quant8<T>(v[i], inv, amax);
+  }
+  for (int c = tid + kQChunks * kQThreads; c < nc; c += kQThreads)
+    out[c] = none ? make_uint2(0, 0) : quant8<T>(row[c], inv, amax);
+}
+
+// ---------------------------------------------------------------- products
+struct GemmParams {
+  const __half* s;
+  const float* sx;
+  const void* res;
+  int64_t ldr;
+  void* c;
+  int64_t ldc;
+  int M, N, K;   // N: output columns (features for SILU)
+  int w3;        // SILU: row of w3 inside W
+  int ntiles;    // pair: tiles along N
+  int n_fast;    // pair: consecutive tiles walk N
+  int vec;       // rows of c and res start on 16 bytes and hold a multiple of 8 columns
+  int m_box;     // small: rows of A that a CTA loads (a multiple of 8)
+  int nst;       // small: ring stages
+  int* err;
+};
+
+constexpr int BK = 128;  // bytes (= int8 elements) of K per stage: one swizzle row
+constexpr int BM = 128;
+
+// kind::i8: D s32, A and B signed 8 bit, K-major
+__host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+HM_DEV void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+HM_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// silu with the fast exponential and quotient (relative error ~2^-21, rounded to 16 bits next)
+HM_DEV float silu_f(float a) { return __fdividef(a, 1.f + __expf(-a)); }
+
+// 8 consecutive columns of TMEM integers, scaled: v * sx * scl
+HM_DEV float scaled(float bits, float sx, float scl) { return static_cast<float>(__float_as_int(bits)) * sx * scl; }
+
+// 16 residual values of one row from column `col` on (zero outside)
+template <typename T>
+HM_DEV void res16(const GemmParams& P, int m, int col, float (&r)[16]) {
+  const T* p = reinterpret_cast<const T*>(P.res) + (int64_t)m * P.ldr + col;
+  if (P.vec && col + 16 <= P.N) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = Ty<T>::f2(u[i]);
+      r[2 * i] = f.x;
+      r[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = col + i < P.N ? Ty<T>::f(p[i]) : 0.f;
+  }
+}
+
+// ---------------------------------------------------------------- few tokens: one tile per CTA
+constexpr int kSmallThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
+constexpr int kMaxStages = 16;
+
+struct SmallBars {
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int BN, int EPI, typename T>
+__global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_constant__ CUtensorMap amap,
+                                                                   const __grid_constant__ CUtensorMap wmap,
+                                                                   const __grid_constant__ GemmParams P) {
+  extern __shared__ uint8_t smem_raw[];  // A stages (m_box rows each), then W stages (BN rows each)
+  uint8_t* const ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ SmallBars sm;
+  __shared__ float scl[BN];
+  constexpr uint32_t kCols = BN < 32 ? 32 : BN;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nt = blockIdx.x, m0 = blockIdx.y * BM;
+  const int nk = (P.K + BK - 1) / BK, nst = P.nst;
+  const uint32_t a_bytes = static_cast<uint32_t>(P.m_box) * BK, w_bytes = BN * BK;
+  uint8_t* const wring = ring + nst * a_bytes;
+  int* const err = P.err;
+  volatile int* abort_s = &sm.abort_flag;
+  if (tid == 0) {
+    sm.abort_flag = 0;
+    for (int i = 0; i < nst; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  constexpr int W = EPI == HM_EPI_SILU ? BN / 2 : BN;  // output columns of the tile
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      prefetch_tensormap(&wmap);
+      prefetch_tensormap(&amap);
+      auto load_w = [&](int kb, int s) {
+        mbar_arrive_expect_tx(&sm.full[s], a_bytes + w_bytes);
+        tma_load_2d_plain(wring + s * w_bytes, &wmap, kb * BK, nt * W, &sm.full[s]);
+        if (EPI == HM_EPI_SILU) tma_load_2d_plain(wring + s * w_bytes + W * BK, &wmap, kb * BK, P.w3 + nt * W, &sm.full[s]);
+      };
+      const int pre = min(nk, nst);
+      for (int kb = 0; kb < pre; ++kb) load_w(kb, kb);  // the weights do not depend on the launch before
+      pdl_wait();
+      for (int kb = 0; kb < pre; ++kb) tma_load_2d_plain(ring + kb * a_bytes, &amap, kb * BK, m0, &sm.full[kb]);
+      for (int kb = pre; kb < nk; ++kb) {
+        const int s = kb % nst;
+        if (!mbar_wait_ab(&sm.empty[s], ((kb / nst) - 1) & 1, err, abort_s)) break;
+        load_w(kb, s);
+        tma_load_2d_plain(ring + s * a_bytes, &amap, kb * BK, m0, &sm.full[s]);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(BM, BN);
+      const uint64_t a0 = sw128_desc(smem_u32(ring)), b0 = sw128_desc(smem_u32(wring));
+      for (int kb = 0; kb < nk; ++kb) {
+        const int s = kb % nst;
+        mbar_wait_ab(&sm.full[s], (kb / nst) & 1, err, abort_s);
+        tc_fence_after();
+        const uint64_t ad = a0 + s * (a_bytes >> 4), bd = b0 + s * (w_bytes >> 4);
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k) umma_i8(tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+        umma_commit(&sm.empty[s]);
+      }
+      umma_commit(&sm.acc_full);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue: a row per thread
+    const int et = tid - 64, quad = warp & 3;  // TMEM lanes 32 * (warp % 4) ..
+    for (int i = et; i < BN; i += 128) {
+      const int col = EPI == HM_EPI_SILU ? nt * W + i % W : nt * W + i;
+      scl[i] = col < P.N ? __half2float(P.s[col + (EPI == HM_EPI_SILU && i >= W ? P.w3 : 0)]) : 0.f;
+    }
+    named_bar(1, 128);
+    const int m = m0 + 32 * quad + lane;
+    pdl_wait();
+    const float sx = m < P.M ? P.sx[m] : 0.f;
+    mbar_wait_ab(&sm.acc_full, 0, err, abort_s);
+    tc_fence_after();
+    if (m0 + 32 * quad < P.M) {  // whole warps (tcgen05.ld is warp-wide)
+      const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quad) << 16);
+      constexpr int STEP = W < 16 ? 8 : 16;
+#pragma unroll 1
+      for (int c0 = 0; c0 < W; c0 += STEP) {
+        __syncwarp();  // rows behind the last one skipped the stores
+        float y[16];
+        if (EPI == HM_EPI_SILU) {
+          float a[16], b[16];
+          if (W < 16) {  // BN = 16: columns 0-7 are w1's, 8-15 w3's
+            tmem_ld16(trow, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = a[8 + i];
+          } else {
+            tmem_ld16(trow + c0, a);
+            tmem_ld16(trow + W + c0, b);
+          }
+#pragma unroll
+          for (int i = 0; i < STEP; ++i)
+            y[i] = silu_f(scaled(a[i], sx, scl[c0 + i])) * scaled(b[i], sx, scl[W + c0 + i]);
+        } else {
+          tmem_ld16(trow + c0, y);
+#pragma unroll
+          for (int i = 0; i < STEP; ++i) y[i] = scaled(y[i], sx, scl[c0 + i]);
+        }
+        const int col = nt * W + c0;
+        if (m >= P.M || col >= P.N) continue;
+        if (EPI != HM_EPI_SILU && P.res) {
+          float r[16];
+          res16<T>(P, m, col, r);
+#pragma unroll
+          for (int i = 0; i < STEP; ++i) y[i] += r[i];
+        }
+        T* c = reinterpret_cast<T*>(P.c) + (int64_t)m * P.ldc + col;
+        if (P.vec && col + STEP <= P.N) {
+#pragma unroll
+          for (int h = 0; h < STEP / 8; ++h)
+            reinterpret_cast<uint4*>(c)[h] =
+                make_uint4(Ty<T>::pack(y[8 * h], y[8 * h + 1]), Ty<T>::pack(y[8 * h + 2], y[8 * h + 3]),
+                           Ty<T>::pack(y[8 * h + 4], y[8 * h + 5]), Ty<T>::pack(y[8 * h + 6], y[8 * h + 7]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < STEP; ++i)
+            if (col + i < P.N) c[i] = Ty<T>::one(y[i]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+// ---------------------------------------------------------------- many tokens: SM pairs
+constexpr int BN2 = 256;
+constexpr int kEpiW = 8;
+constexpr int kPairThreads = 64 + 32 * kEpiW;
+constexpr int NS2 = 5;
+constexpr int kTileBytes = BM * BK;  // 16 KB: 128 rows of A, or a CTA's half of the weight tile
+
+struct PairSmem {
+  uint8_t a[NS2][kTileBytes];
+  uint8_t b[NS2][kTileBytes];
+  uint8_t stage[BM * 512];  // 128 rows x 256 results
+  __half scl[2][BN2];
+  uint64_t full[NS2], empty[NS2];      // full: used in the leader CTA only
+  uint64_t acc_full[2], acc_empty[2];  // acc_empty: the leader's, the epilogue warps of both CTAs arrive
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// The tile's results: warp w reads TMEM lanes 32 * (w % 4) .. +31 over half of the columns, scales
+// (SiLU, residual), rounds and stages them (16-byte chunk c of row r at slot c ^ (r & 7)); then it
+// copies its 32 rows out as whole row segments.  `release` hands the accumulator back.
+template <int EPI, typename T, typename Release>
+HM_DEV void pair_epilogue(const GemmParams& P, uint32_t tmem, int warp, int lane, int m_row0, int nt, uint8_t* stage,
+                          __half* scl, Release release) {
+  const int et = (warp - 2) * 32 + lane, quad = warp & 3, part = (warp - 2) / 4;
+  constexpr int WT = EPI == HM_EPI_SILU ? BN2 / 2 : BN2;  // output columns of the tile
+  constexpr int W = WT / 2;                               // of this warp
+  constexpr int cpr = W / 8, rpi = 32 / cpr;              // 16-byte chunks per row, rows per copy step
+  const int col0 = nt * WT;
+  {
+    const int col = EPI == HM_EPI_SILU ? col0 + (et & (WT - 1)) : col0 + et;
+    scl[et] = col < P.N ? P.s[col + (EPI == HM_EPI_SILU && et >= WT ? P.w3 : 0)] : __float2half_rn(0.f);
+  }
+  named_bar(1, 32 * kEpiW);
+  const int r = 32 * quad + lane, m = m_row0 + r;
+  const float sx = m < P.M ? P.sx[m] : 0.f;
+  const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quad) << 16);
+  uint8_t* const srow = stage + r * 512;
+#pragma unroll 1
+  for (int c0 = part * W; c0 < (part + 1) * W; c0 += 16) {
+    float y[16];
+    if (EPI == HM_EPI_SILU) {
+      float a[16], b[16];
+      tmem_ld16(trow + c0, a);
+      tmem_ld16(trow + BN2 / 2 + c0, b);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        y[i] = silu_f(scaled(a[i], sx, __half2float(scl[c0 + i]))) *
+               scaled(b[i], sx, __half2float(scl[BN2 / 2 + c0 + i]));
+    } else {
+      float rr[16];
+      const bool add = P.res && m < P.M && col0 + c0 < P.N;
+      if (add) res16<T>(P, m, col0 + c0, rr);
+      __syncwarp();
+      tmem_ld16(trow + c0, y);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = scaled(y[i], sx, __half2float(scl[c0 + i])) + (add ? rr[i] : 0.f);
+    }
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = Ty<T>::pack(y[2 * i], y[2 * i + 1]);
+    const int ch = c0 / 8;
+    *reinterpret_cast<uint4*>(srow + ((ch ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(srow + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+  release();
+  __syncwarp();
+  T* const C = reinterpret_cast<T*>(P.c);
+#pragma unroll 4
+  for (int it = 0; it < 32 / rpi; ++it) {
+    const int rr = 32 * quad + it * rpi + lane / cpr, ch = part * cpr + lane % cpr;
+    const int mm = m_row0 + rr, col = col0 + 8 * ch;
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 512 + ((ch ^ (rr & 7)) << 4));
+    if (mm >= P.M || col >= P.N) continue;
+    T* c = C + (int64_t)mm * P.ldc + col;
+    if (P.vec) {
+      *reinterpret_cast<uint4*>(c) = v;
+    } else {
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < P.N) c[i] = e[i];
+    }
+  }
+}
+
+static_assert(sizeof(PairSmem) + 1024 <= 227 * 1024, "one CTA per SM");
+
+template <int EPI, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap,
+                     const __grid_constant__ GemmParams P) {
+  extern __shared__ uint8_t smem_raw[];
+  PairSmem& sm = *reinterpret_cast<PairSmem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = static_cast<int>(blockIdx.x >> 1), npairs = static_cast<int>(gridDim.x >> 1);
+  const int mpairs = (P.M + 2 * BM - 1) / (2 * BM), tiles = mpairs * P.ntiles;
+  const int nk = (P.K + BK - 1) / BK;
+  int* const err = P.err;
+  constexpr int WT = EPI == HM_EPI_SILU ? BN2 / 2 : BN2;
+  if (tid == 0) {
+    sm.abort_flag = 0;
+    for (int i = 0; i < NS2; ++i) {
+      mbar_init(&sm.full[i], 1);   // the leader's producer (expect_tx) + both CTAs' copies (bytes)
+      mbar_init(&sm.empty[i], 1);  // the leader's MMA commit
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.acc_full[i], 1);
+      mbar_init(&sm.acc_empty[i], 2 * kEpiW);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc_pair(&sm.tmem_base, 2 * BN2);
+  tc_fence_before();
+  cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* abort_s = &sm.abort_flag;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      prefetch_tensormap(&amap);
+      prefetch_tensormap(&wmap);
+      const uint32_t full0 = dsmem_addr(&sm.full[0], 0);
+      int g = 0;
+      for (int t = pair; t < tiles; t += npairs) {
+        const int mp = P.n_fast ? t / P.ntiles : t % mpairs, nt = P.n_fast ? t % P.ntiles : t / mpairs;
+        const int m_row0 = mp * 2 * BM + static_cast<int>(rank) * BM;
+        const int brow = EPI == HM_EPI_SILU ? (rank == 0 ? 0 : P.w3) + nt * WT : nt * WT + static_cast<int>(rank) * BM;
+        for (int kb = 0; kb < nk; ++kb, ++g) {
+          const int s = g % NS2;
+          if (g >= NS2) mbar_wait_ab(&sm.empty[s], ((g / NS2) - 1) & 1, err, abort_s);
+          if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kTileBytes);
+          tma_load_2d_pair(sm.a[s], &amap, kb * BK, m_row0, full0 + 8 * s);
+          tma_load_2d_pair(sm.b[s], &wmap, kb * BK, brow, full0 + 8 * s);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader CTA)
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_i8(2 * BM, BN2);
+      const uint64_t a0 = sw128_desc(smem_u32(sm.a[0])), b0 = sw128_desc(smem_u32(sm.b[0]));
+      int g = 0, i = 0;
+      for (int t = pair; t < tiles; t += npairs, ++i) {
+        const int ab = i & 1;
+        if (i >= 2 && !*abort_s && !mbar_wait_cluster(&sm.acc_empty[ab], ((i >> 1) - 1) & 1, err)) *abort_s = 1;
+        tc_fence_after();
+        const uint32_t acc = tmem + ab * BN2;
+        for (int kb = 0; kb < nk; ++kb, ++g) {
+          const int s = g % NS2;
+          mbar_wait_ab(&sm.full[s], (g / NS2) & 1, err, abort_s);
+          tc_fence_after();
+          const uint64_t ad = a0 + s * (kTileBytes >> 4), bd = b0 + s * (kTileBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k) umma_i8_pair(acc, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+          umma_commit_pair(&sm.empty[s]);
+        }
+        umma_commit_pair(&sm.acc_full[ab]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs: their 128 rows)
+    const uint32_t acc_empty0 = dsmem_addr(&sm.acc_empty[0], 0);
+    int i = 0;
+    for (int t = pair; t < tiles; t += npairs, ++i) {
+      const int ab = i & 1;
+      const int mp = P.n_fast ? t / P.ntiles : t % mpairs, nt = P.n_fast ? t % P.ntiles : t / mpairs;
+      const int m_row0 = mp * 2 * BM + static_cast<int>(rank) * BM;
+      mbar_wait_ab(&sm.acc_full[ab], (i >> 1) & 1, err, abort_s);
+      tc_fence_after();
+      pair_epilogue<EPI, T>(P, tmem + ab * BN2, warp, lane, m_row0, nt, sm.stage, sm.scl[ab], [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0)
+            mbar_arrive(&sm.acc_empty[ab]);
+          else
+            mbar_arrive_dsmem(acc_empty0 + 8 * ab);
+        }
+      });
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA leaves while the pair's copies, MMAs or commits may touch its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 2 * BN2);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int kMaxDevices = 64;
+
+cudaError_t device_sms(int* dev, int* sms) {
+  static std::atomic<int> known[kMaxDevices];
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return e;
+  if (*dev < kMaxDevices && (*sms = known[*dev].load()) > 0) return cudaSuccess;
+  e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev);
+  if (e == cudaSuccess && *dev < kMaxDevices) known[*dev].store(*sms);
+  return e;
+}
+
+// int8 [rows, cols] with a row pitch of ld bytes: boxes of 128 bytes x box_rows, 128-byte swizzle
+bool tile_map(const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows, CUtensorMap* out) {
+  auto enc = hm_encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {BK, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t es[2] = {1, 1};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K>
+cudaError_t max_smem(K kernel, std::atomic<bool>* configured, int dev, size_t bytes) {
+  if (dev < kMaxDevices && configured[dev].load()) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && dev < kMaxDevices) configured[dev].store(true);
+  return e;
+}
+
+constexpr int kSmallRing = 106 * 1024;  // a small CTA's ring: two CTAs per SM
+
+template <int BN, int EPI, typename T>
+cudaError_t launch_small(const CUtensorMap& am, const CUtensorMap& wm, GemmParams p, int dev, int pdl, cudaStream_t st) {
+  static std::atomic<bool> configured[kMaxDevices];
+  cudaError_t e = max_smem(gemm_small_kernel<BN, EPI, T>, configured, dev, kSmallRing + 1024);
+  if (e != cudaSuccess) return e;
+  const int stage = (p.m_box + BN) * BK, nk = (p.K + BK - 1) / BK;
+  p.nst = kSmallRing / stage < kMaxStages ? kSmallRing / stage : kMaxStages;
+  if (p.nst > nk) p.nst = nk;
+  // at the last A stage the MMA reads 128 rows: they have to lie inside the allocation
+  const int reach = (p.nst - 1) * p.m_box * BK + BM * BK, ring = p.nst * stage > reach ? p.nst * stage : reach;
+  static_assert(kSmallRing / ((BM + 128) * BK) >= 3 && 2 * kSmallRing + 6 * 1024 <= 228 * 1024, "ring");
+  constexpr int W = EPI == HM_EPI_SILU ? BN / 2 : BN;
+  const dim3 grid((p.N + W - 1) / W, (p.M + BM - 1) / BM);
+  return hm_launch(gemm_small_kernel<BN, EPI, T>, grid, dim3(kSmallThreads), static_cast<size_t>(ring) + 1024, st, pdl, am, wm, p);
+}
+
+template <int EPI, typename T>
+cudaError_t launch_pair(const CUtensorMap& am, const CUtensorMap& wm, GemmParams p, int sms, int dev, int pdl,
+                        cudaStream_t st) {
+  static std::atomic<bool> configured[kMaxDevices];
+  constexpr size_t smem = sizeof(PairSmem) + 1024;
+  const cudaError_t e = max_smem(gemm_pair_kernel<EPI, T>, configured, dev, smem);
+  if (e != cudaSuccess) return e;
+  constexpr int WT = EPI == HM_EPI_SILU ? BN2 / 2 : BN2;
+  p.ntiles = (p.N + WT - 1) / WT;
+  p.n_fast = p.M > (EPI == HM_EPI_SILU ? 2 * p.N : p.N);
+  const int64_t tiles = (int64_t)((p.M + 2 * BM - 1) / (2 * BM)) * p.ntiles;
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  return hm_launch(gemm_pair_kernel<EPI, T>, dim3(2 * pairs), dim3(kPairThreads), smem, st, pdl, am, wm, p);
+}
+
+template <int EPI, typename T>
+cudaError_t launch_gemm(const int8_t* q, int64_t ldq, const int8_t* w, GemmParams p, int wrows, int pdl, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  cudaError_t e = device_sms(&dev, &sms);
+  if (e != cudaSuccess) return e;
+  CUtensorMap am, wm;
+  const int64_t pair_tiles = (int64_t)((p.M + 255) / 256) * ((wrows + 255) / 256);
+  if (p.M > BM && pair_tiles >= sms / 4) {
+    if (!tile_map(q, p.M, p.K, ldq, BM, &am) || !tile_map(w, wrows, p.K, p.K, BM, &wm)) return cudaErrorInvalidValue;
+    return launch_pair<EPI, T>(am, wm, p, sms, dev, pdl, st);
+  }
+  const int mt = (p.M + BM - 1) / BM;
+  p.m_box = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
+  // the widest tile whose grid takes the fewest columns per SM
+  int bn = 128;
+  int64_t best = INT64_MAX;
+  for (int b = 128; b >= 16; b /= 2) {
+    const int64_t tiles = (int64_t)mt * ((wrows + b - 1) / b), cost = (tiles + sms - 1) / sms * b;
+    if (cost < best) {
+      best = cost;
+      bn = b;
+    }
+  }
+  if (!tile_map(q, p.M, p.K, ldq, p.m_box, &am) ||
+      !tile_map(w, wrows, p.K, p.K, EPI == HM_EPI_SILU ? bn / 2 : bn, &wm))
+    return cudaErrorInvalidValue;
+  switch (bn) {
+    case 128: return launch_small<128, EPI, T>(am, wm, p, dev, pdl, st);
+    case 64: return launch_small<64, EPI, T>(am, wm, p, dev, pdl, st);
+    case 32: return launch_small<32, EPI, T>(am, wm, p, dev, pdl, st);
+    default: return launch_small<16, EPI, T>(am, wm, p, dev, pdl, st);
+  }
+}
+
+bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u); }
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+bool x_ok(const void* x, int64_t ldx, int dtype, int M, int K) {
+  return !bad16(x) && (dtype == HM_DT_F16 || dtype == HM_DT_BF16) && M >= 1 && K >= 16 && K % 16 == 0 && K <= 131072 &&
+         ldx >= K && ldx % 8 == 0;
+}
+
+bool out_ok(const int8_t* w, const void* s, const void* res, int64_t ldr, const void* c, int64_t ldc, int N, int epi) {
+  if (bad16(w) || !s || !c || N < 1 || (epi != HM_EPI_STORE && epi != HM_EPI_SILU)) return false;
+  if (epi == HM_EPI_SILU && (res || N % 2)) return false;
+  const int nout = epi == HM_EPI_SILU ? N / 2 : N;
+  return ldc >= nout && (!res || ldr >= nout) && !(reinterpret_cast<uintptr_t>(s) & 1u) &&
+         !(reinterpret_cast<uintptr_t>(c) & 1u) && !(reinterpret_cast<uintptr_t>(res) & 1u);
+}
+
+template <typename T>
+cudaError_t quantise(const void* x, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* sx, cudaStream_t st) {
+  return hm_launch(quant_kernel<T>, dim3(M), dim3(kQThreads), 0, st, 0, reinterpret_cast<const T*>(x), ldx, K, q, ldq, sx);
+}
+
+cudaError_t multiply(const int8_t* q, int64_t ldq, const float* sx, int dtype, const int8_t* w, const void* s,
+                     const void* res, int64_t ldr, void* c, int64_t ldc, int M, int N, int K, int epi, int* err, int pdl,
+                     cudaStream_t st) {
+  GemmParams p = {};
+  p.s = reinterpret_cast<const __half*>(s);
+  p.sx = sx;
+  p.res = res;
+  p.ldr = ldr;
+  p.c = c;
+  p.ldc = ldc;
+  p.M = M;
+  p.N = epi == HM_EPI_SILU ? N / 2 : N;
+  p.K = K;
+  p.w3 = epi == HM_EPI_SILU ? N / 2 : 0;
+  p.vec = p.N % 8 == 0 && ldc % 8 == 0 && !off16(c) && (!res || (ldr % 8 == 0 && !off16(res)));
+  p.err = err;
+  if (epi == HM_EPI_SILU)
+    return dtype == HM_DT_F16 ? launch_gemm<HM_EPI_SILU, __half>(q, ldq, w, p, N, pdl, st)
+                              : launch_gemm<HM_EPI_SILU, __nv_bfloat16>(q, ldq, w, p, N, pdl, st);
+  return dtype == HM_DT_F16 ? launch_gemm<HM_EPI_STORE, __half>(q, ldq, w, p, N, pdl, st)
+                            : launch_gemm<HM_EPI_STORE, __nv_bfloat16>(q, ldq, w, p, N, pdl, st);
+}
+
+int rc_of(cudaError_t e) { return e == cudaSuccess ? HM_OK : static_cast<int>(e); }
+
+size_t scale_bytes(int M) { return ((size_t)M * sizeof(float) + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" int hm_quant_tokens(const void* x, int64_t ldx, int dtype, int M, int K, int8_t* q, int64_t ldq, float* sx,
+                               hm_stream_t stream) {
+  if (!x_ok(x, ldx, dtype, M, K) || bad16(q) || !sx || (reinterpret_cast<uintptr_t>(sx) & 3u) || ldq < K || ldq % 8)
+    return HM_EARG;
+  return rc_of(dtype == HM_DT_F16 ? quantise<__half>(x, ldx, M, K, q, ldq, sx, stream)
+                                  : quantise<__nv_bfloat16>(x, ldx, M, K, q, ldq, sx, stream));
+}
+
+extern "C" int hm_gemm_i8a8(const int8_t* q, int64_t ldq, const float* sx, int dtype, const int8_t* w, const void* s,
+                            const void* res, int64_t ldr, void* c, int64_t ldc, int M, int N, int K, int epi, int* err,
+                            hm_stream_t stream) {
+  if (bad16(q) || ldq < K || ldq % 16 || !sx || (reinterpret_cast<uintptr_t>(sx) & 3u) || M < 1 || K < 16 || K % 16 ||
+      K > 131072 || (dtype != HM_DT_F16 && dtype != HM_DT_BF16) || !out_ok(w, s, res, ldr, c, ldc, N, epi))
+    return HM_EARG;
+  return rc_of(multiply(q, ldq, sx, dtype, w, s, res, ldr, c, ldc, M, N, K, epi, err, 0, stream));
+}
+
+extern "C" size_t hm_int8_mm_a8_workspace_bytes(int M, int K) {
+  return M < 1 || K < 1 ? 0 : scale_bytes(M) + (size_t)M * K;
+}
+
+extern "C" int hm_int8_mm_a8(const void* x, int64_t ldx, int dtype, const int8_t* w, const void* s, const void* res,
+                             int64_t ldr, void* c, int64_t ldc, int M, int N, int K, int epi, void* ws, size_t ws_bytes,
+                             int* err, hm_stream_t stream) {
+  if (!x_ok(x, ldx, dtype, M, K) || !out_ok(w, s, res, ldr, c, ldc, N, epi) || bad16(ws) ||
+      ws_bytes < hm_int8_mm_a8_workspace_bytes(M, K))
+    return HM_EARG;
+  float* sx = reinterpret_cast<float*>(ws);
+  int8_t* q = reinterpret_cast<int8_t*>(ws) + scale_bytes(M);
+  cudaError_t e = dtype == HM_DT_F16 ? quantise<__half>(x, ldx, M, K, q, K, sx, stream)
+                                     : quantise<__nv_bfloat16>(x, ldx, M, K, q, K, sx, stream);
+  // the product may start beside the quantisation: that launch waits for everything before it, and
+  // the product reads only the weights and their scales before it waits in turn
+  if (e == cudaSuccess) e = multiply(q, K, sx, dtype, w, s, res, ldr, c, ldc, M, N, K, epi, err, 1, stream);
+  return rc_of(e);
+}

@@ -517,6 +517,96 @@ def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int 
     return o
 
 
+# ----------------------------------------------------------------------------- 8-bit integer product
+def _rows16(what: str, x) -> torch.Tensor:
+    """x ``[M, K]`` fp16 or bf16 with 16-byte rows (copied when its rows do not start on 16 bytes)."""
+    if x.dtype not in _DT or x.dim() != 2 or x.shape[0] < 1:
+        raise HMError(f"{what}: fp16 or bf16 rows [M, K]")
+    K = x.shape[1]
+    if K < 16 or K % 16 or K > 131072:
+        raise HMError(f"{what}: K a multiple of 16, at most 131072")
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < K)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _pitch(t) -> int:
+    """Row pitch of a 2-D tensor (a single row's stride may be anything)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _a8_out(what: str, dtype, w, s, res, out, silu: bool, M: int, K: int, device):
+    """Checks of the weights and outputs; returns (N, out)."""
+    if w.dtype != torch.int8 or w.dim() != 2 or w.shape[1] != K or w.shape[0] < 1 or not w.is_contiguous():
+        raise HMError(f"{what}: w is contiguous int8 [N, K]")
+    N = w.shape[0]
+    if s.dtype != torch.float16 or s.dim() != 1 or s.numel() != N or not s.is_contiguous():
+        raise HMError(f"{what}: s is fp16 [N]")
+    if silu and (res is not None or N % 2):
+        raise HMError(f"{what}: silu takes w = [w1; w3] and no residual")
+    nout = N // 2 if silu else N
+    if res is not None and (res.dtype != dtype or not _is_rows(res, M, nout)):
+        raise HMError(f"{what}: res [M, N] of the activations' type")
+    if out is None:
+        out = torch.empty(M, nout, dtype=dtype, device=device)
+    elif out.dtype != dtype or not _is_rows(out, M, nout):
+        raise HMError(f"{what}: out [M, N] of the activations' type")
+    return N, out
+
+
+def quant_tokens(x: torch.Tensor):
+    """Per-token int8: ``(q int8 [M, K], sx float32 [M])`` with ``sx = max|x| / 127`` and ``q`` the exact
+    quotient ``x / sx`` rounded half to even.  A row with an infinity or NaN gets ``q = 0``, ``sx = NaN``."""
+    idx = _device_of("quant_tokens", x)
+    x = _rows16("quant_tokens", x)
+    M, K = x.shape
+    q = torch.empty(M, K, dtype=torch.int8, device=x.device)
+    sx = torch.empty(M, dtype=torch.float32, device=x.device)
+    _launch(idx, "hm_quant_tokens", x.data_ptr(), _pitch(x), _DT[x.dtype], M, K, q.data_ptr(), K, sx.data_ptr())
+    return q, sx
+
+
+def gemm_i8a8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, s: torch.Tensor, res: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, silu: bool = False, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """:func:`gemm_i8w` with the activations in 8 bits: ``q [M, K]`` int8 and ``sx [M]`` from
+    :func:`quant_tokens` times int8 ``w [N, K]`` with per-row scales, on the tensor cores in exact
+    integers; scales, residual and SiLU in fp32, one rounding to ``dtype`` (fp16 or bf16).  ``res`` may
+    be ``out``."""
+    idx = _device_of("gemm_i8a8", q, sx, w, s, res, out)
+    if q.dtype != torch.int8 or q.dim() != 2 or q.stride(1) != 1 or dtype not in _DT:
+        raise HMError("gemm_i8a8: q int8 [M, K], dtype fp16 or bf16")
+    M, K = q.shape
+    if sx.dtype != torch.float32 or sx.dim() != 1 or sx.numel() != M or not sx.is_contiguous():
+        raise HMError("gemm_i8a8: sx is float32 [M]")
+    N, out = _a8_out("gemm_i8a8", dtype, w, s, res, out, silu, M, K, q.device)
+    _launch(idx, "hm_gemm_i8a8", q.data_ptr(), _pitch(q), sx.data_ptr(), _DT[dtype], w.data_ptr(), s.data_ptr(),
+            None if res is None else res.data_ptr(), 0 if res is None else _pitch(res), out.data_ptr(), _pitch(out), M,
+            N, K, _lib.HM_EPI_SILU if silu else _lib.HM_EPI_STORE, _err_ptr(idx))
+    return out
+
+
+def int8_mm_a8(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, res: torch.Tensor | None = None,
+               silu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`int8_mm` with the activations quantised per token first (:func:`quant_tokens`), for any
+    number of rows: ``x [..., K]`` fp16 or bf16 -> ``[..., N]`` (``[..., N / 2]`` with ``silu``, ``w`` the
+    fused w1|w3) of x's type (+ ``res``).  ``out`` ``[rows, N]`` may be ``res``."""
+    idx = _device_of("int8_mm_a8", x, w, s, res, out)
+    shp = x.shape
+    flat = len(shp) != 2
+    if flat:
+        x = x.reshape(-1, shp[-1])
+        res = None if res is None else res.reshape(x.shape[0], -1)
+    x = _rows16("int8_mm_a8", x)
+    M, K = x.shape
+    N, out = _a8_out("int8_mm_a8", x.dtype, w, s, res, out, silu, M, K, x.device)
+    nbytes = _lib.lib().hm_int8_mm_a8_workspace_bytes(M, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _launch(idx, "hm_int8_mm_a8", x.data_ptr(), _pitch(x), _DT[x.dtype], w.data_ptr(), s.data_ptr(),
+            None if res is None else res.data_ptr(), 0 if res is None else _pitch(res), out.data_ptr(), _pitch(out), M,
+            N, K, _lib.HM_EPI_SILU if silu else _lib.HM_EPI_STORE, ws.data_ptr(), nbytes, _err_ptr(idx))
+    return out.reshape(*shp[:-1], out.shape[1]) if flat else out
+
+
 # ----------------------------------------------------------------------------- raw-launch stand-ins
 class _Launch:
     """A kernel name that launches with the reference's ``kernel[grid](*args, **meta)``

@@ -275,6 +275,27 @@ int hm_gemm_f16w(const void* a, int64_t lda, const void* w, const void* s, const
  * (app/kernels.py:46-49) without the scale, which hm_gemm_f16w applies to the sums. */
 int hm_dequant_i8_f16(const int8_t* w, void* out, int64_t n, hm_stream_t stream);
 
+/* Matrix product in 8-bit integers with a scale for each token and each output channel: int8_mm
+ * (app/kernels.py:40-54) with the activations in 8 bits too.
+ * hm_quant_tokens: sx[m] = max_k |x[m, k]| / 127, q[m, k] = x / sx[m] rounded half to even from the
+ *   exact quotient (a zero row: zeros; a row with an infinity or NaN: q = 0, sx = NaN).
+ * hm_gemm_i8a8: acc = sum_k q[m, k] * w[n, k] (exact), fp32 from there, one rounding to dtype:
+ *   epi HM_EPI_STORE: c[m, n] = acc * sx[m] * s[n] (+ res[m, n]);   c may equal res
+ *   epi HM_EPI_SILU : w = [w1; w3] (N = 2F rows), c[m, f] = silu(a) * b  (res must be NULL)
+ * hm_int8_mm_a8: both, for x as it comes (ws: hm_int8_mm_a8_workspace_bytes, 16-byte aligned).
+ * dtype HM_DT_F16 or HM_DT_BF16 (x, res, c); s fp16 [N]; any M and N >= 1 (rows of 8 columns on
+ * 16 bytes are stored as vectors); K % 16 == 0, K <= 131072; x, q, w 16-byte aligned, ldx % 8 == 0,
+ * ldq % 8 == 0 (16 for hm_gemm_i8a8). */
+int hm_quant_tokens(const void* x, int64_t ldx, int dtype, int M, int K, int8_t* q, int64_t ldq, float* sx,
+                    hm_stream_t stream);
+int hm_gemm_i8a8(const int8_t* q, int64_t ldq, const float* sx, int dtype, const int8_t* w, const void* s,
+                 const void* res, int64_t ldr, void* c, int64_t ldc, int M, int N, int K, int epi, int* err,
+                 hm_stream_t stream);
+int hm_int8_mm_a8(const void* x, int64_t ldx, int dtype, const int8_t* w, const void* s, const void* res, int64_t ldr,
+                  void* c, int64_t ldc, int M, int N, int K, int epi, void* ws, size_t ws_bytes, int* err,
+                  hm_stream_t stream);
+size_t hm_int8_mm_a8_workspace_bytes(int M, int K);
+
 /* Causal GQA attention of a whole prompt over the cache positions [0, P) that the
  * RoPE/KV-write step filled: q, o [B*P, Hq*hd] fp16 (row b*P + p), kc/vc [B, Hk, L, hd].
  * hd == 128, Hq/Hk <= 4.  Replaces the prompt branch of Block.__call__'s attention

@@ -86,3 +86,25 @@ def test_prefix_attn(lib):
     ws = lib.hm_prefix_attn_workspace_bytes
     assert ws(4, 1, 8, 2, 128, 1, 148) > 0 and ws(4, 1, 8, 2, 96, 1, 148) == 0 and ws(4, 3, 8, 2, 128, 1, 148) == 0
     assert ws(8, 1, 65 * 2, 2, 128, 1, 148) == 0
+
+
+def test_integer_product(lib):
+    quant = dict(x=16, ldx=128, dt=2, M=4, K=128, q=16, ldq=128, sx=16, st=None)
+    for kw in (dict(x=None), dict(x=24), dict(ldx=120), dict(ldx=132), dict(dt=0), dict(M=0), dict(K=0), dict(K=120),
+               dict(K=131088, ldx=131088, ldq=131088), dict(q=None), dict(q=24), dict(ldq=120), dict(ldq=130), dict(sx=None),
+               dict(sx=18)):
+        assert lib.hm_quant_tokens(*{**quant, **kw}.values()) == -1, kw
+    gemm = dict(q=16, ldq=128, sx=16, dt=2, w=16, s=16, res=None, ldr=0, c=16, ldc=64, M=4, N=64, K=128, epi=0, err=None,
+                st=None)
+    for kw in (dict(q=None), dict(q=24), dict(ldq=120), dict(ldq=136), dict(sx=None), dict(dt=0), dict(w=24), dict(w=None),
+               dict(s=None), dict(s=17), dict(res=16, ldr=63), dict(res=17, ldr=64), dict(c=None), dict(c=17), dict(ldc=63),
+               dict(M=0), dict(N=0), dict(K=8), dict(K=100), dict(K=131088), dict(epi=1), dict(epi=2, N=63),
+               dict(epi=2, res=16, ldr=64)):
+        assert lib.hm_gemm_i8a8(*{**gemm, **kw}.values()) == -1, kw
+    mm = dict(x=16, ldx=128, dt=2, w=16, s=16, res=None, ldr=0, c=16, ldc=64, M=4, N=64, K=128, epi=0, ws=16, wsb=1 << 20,
+              err=None, st=None)
+    for kw in (dict(x=None), dict(ldx=120), dict(dt=0), dict(w=None), dict(c=17), dict(ldc=10), dict(K=24, ldx=24), dict(M=0),
+               dict(ws=None), dict(ws=24), dict(wsb=lib.hm_int8_mm_a8_workspace_bytes(4, 128) - 1), dict(epi=2, N=7)):
+        assert lib.hm_int8_mm_a8(*{**mm, **kw}.values()) == -1, kw
+    assert lib.hm_int8_mm_a8_workspace_bytes(0, 128) == 0
+    assert lib.hm_int8_mm_a8_workspace_bytes(65, 128) == 512 + 65 * 128

@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import gc
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libheartmula_b200.so"
@@ -82,6 +83,13 @@ class PrefixAttnDesc(C.Structure):
                 ("n_groups", C.c_int), ("scale", C.c_float)]
 
 
+# The same three descriptors as packed bytes (native alignment, trailing padding included): a call
+# takes the bytes object as the pointer, which costs a quarter of filling a ctypes structure.
+PACK_PAGE_STATE = struct.Struct("@PqPPP4i0P")
+PACK_PAGE_POOL = struct.Struct("@PP5i0P")
+PACK_PREFIX_ATTN = struct.Struct("@PqPqPPPPqPPPPPNP11if0P")
+
+
 SIGNATURES = {
     "hm_gemv_i8": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _P, _SZ, _P, _I, _P, _I, _I, _P]),
     "hm_gemv_i8_fused": (_I, [C.POINTER(GemvDesc), _P]),
@@ -108,14 +116,14 @@ SIGNATURES = {
     "hm_gemm_i8a8": (_I, [_P, _I64, _P, _I, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P]),
     "hm_int8_mm_a8": (_I, [_P, _I64, _I, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _SZ, _P, _P]),
     "hm_int8_mm_a8_workspace_bytes": (_SZ, [_I, _I]),
-    "hm_prefix_attn": (_I, [C.POINTER(PrefixAttnDesc), _P]),
+    "hm_prefix_attn": (_I, [_P, _P]),
     "hm_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "hm_pages_workspace_bytes": (_SZ, [_I, _I]),
-    "hm_pages_grow": (_I, [C.POINTER(PageState), _P, _I, _I, _P]),
-    "hm_pages_free": (_I, [C.POINTER(PageState), _P, _I, _P]),
-    "hm_pages_fork": (_I, [C.POINTER(PageState), C.POINTER(PagePoolDesc), _P, _P, _I, _P, _SZ, _P]),
-    "hm_pages_copy": (_I, [C.POINTER(PagePoolDesc), _P, _P, _I, _P, _SZ, _P, _P]),
-    "hm_pages_compact": (_I, [C.POINTER(PageState), C.POINTER(PagePoolDesc), _P, _P, _SZ, _P]),
+    "hm_pages_grow": (_I, [_P, _P, _I, _I, _P]),
+    "hm_pages_free": (_I, [_P, _P, _I, _P]),
+    "hm_pages_fork": (_I, [_P, _P, _P, _P, _I, _P, _SZ, _P]),
+    "hm_pages_copy": (_I, [_P, _P, _P, _I, _P, _SZ, _P, _P]),
+    "hm_pages_compact": (_I, [_P, _P, _P, _P, _SZ, _P]),
     "hm_rope_pages": (_I, [_P, _I64, _P, _I, _P, _P, _I64, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                            _P, _P]),
     "hm_conv1d_gemm": (_I, [C.POINTER(ConvDesc), _P]),
@@ -210,4 +218,7 @@ def abi_mismatches() -> list[str]:
             8: ConvDesc.scale.offset, 9: ConvDesc.bn.offset, 10: C.sizeof(PageState), 11: PageState.page.offset,
             12: C.sizeof(PagePoolDesc), 13: PagePoolDesc.row_bytes.offset,
             14: C.sizeof(PrefixAttnDesc), 15: PrefixAttnDesc.scale.offset}
-    return [f"layout[{k}]: C {L.hm_abi_layout(k)} vs ctypes {v}" for k, v in want.items() if L.hm_abi_layout(k) != v]
+    bad = [f"layout[{k}]: C {L.hm_abi_layout(k)} vs ctypes {v}" for k, v in want.items() if L.hm_abi_layout(k) != v]
+    bad += [f"packed size {p.size} vs {C.sizeof(t)}" for p, t in ((PACK_PAGE_STATE, PageState), (PACK_PAGE_POOL, PagePoolDesc),
+                                                                  (PACK_PREFIX_ATTN, PrefixAttnDesc)) if p.size != C.sizeof(t)]
+    return bad

@@ -16,7 +16,7 @@
 //
 // Two products, both tcgen05.mma kind::i8 (K = 32 a step) fed by TMA (128-byte swizzle, K blocks of
 // 128 bytes) with the int32 sums in TMEM:
-//  * gemm_small: one 128 x BN tile per CTA, BN = 16 .. 128.  For few tokens the weights are all the
+//  * gemm_small: one MT x BN tile per CTA, MT = 64 or 128, BN = 32 .. 128.  For few tokens the weights are all the
 //    traffic, so BN is chosen to put the weight stream on as many SMs as there are, and a CTA
 //    keeps a ring of up to ~100 KB in flight.  Only the rows that exist are loaded: the MMA's
 //    other rows read whatever lies behind them in shared memory, and nobody reads their sums.
@@ -59,15 +59,18 @@ struct Ty<__nv_bfloat16> {
 };
 
 // ---------------------------------------------------------------- quantisation of the tokens
-constexpr int kQThreads = 256;
-constexpr int kQChunks = 8;  // 8-element chunks a thread keeps in registers (K <= 16384)
+constexpr int kQChunks = 4;  // 8-element chunks a thread keeps in registers (K <= 32 * threads)
 
-HM_DEV int quant1(float x, float inv, float amax) {
-  const float t = x * inv;
-  float r = rintf(t);
+// Adding 1.5 * 2^23 rounds a small value half to even into the low mantissa bits, whose last byte is
+// the integer's: no conversion instructions (they run at an eighth of the adds' rate).
+constexpr float kRound = 12582912.f;
+
+HM_DEV uint32_t quant1(float x, float inv, float amax) {
+  const float t = __fmul_rn(x, inv), r = __fadd_rn(t, kRound);
   // near a half (or an overflowing reciprocal): the exact quotient decides
-  if (!(fabsf(t - r) < 0.5f - 3.0517578125e-5f)) r = rintf(__fdiv_rn(x * 127.f, amax));
-  return static_cast<int>(r);
+  if (!(fabsf(__fsub_rn(t, __fsub_rn(r, kRound))) < 0.5f - 3.0517578125e-5f))
+    return __float_as_uint(__fadd_rn(__fdiv_rn(__fmul_rn(x, 127.f), amax), kRound));
+  return __float_as_uint(r);
 }
 
 template <typename T>
@@ -77,8 +80,8 @@ HM_DEV uint2 quant8(uint4 v, float inv, float amax) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const float2 a = Ty<T>::f2(u[2 * h]), b = Ty<T>::f2(u[2 * h + 1]);
-    out[h] = (quant1(a.x, inv, amax) & 0xff) | ((quant1(a.y, inv, amax) & 0xff) << 8) |
-             ((quant1(b.x, inv, amax) & 0xff) << 16) | (static_cast<uint32_t>(quant1(b.y, inv, amax)) << 24);
+    out[h] = __byte_perm(__byte_perm(quant1(a.x, inv, amax), quant1(a.y, inv, amax), 0x0040),
+                         __byte_perm(quant1(b.x, inv, amax), quant1(b.y, inv, amax), 0x0040), 0x5410);
   }
   return make_uint2(out[0], out[1]);
 }
@@ -91,10 +94,10 @@ HM_DEV uint32_t top_bits(uint4 v, uint32_t top) {
   return top;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kQThreads) quant_kernel(const T* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
-                                                          int64_t ldq, float* __restrict__ sx) {
-  __shared__ uint32_t red[kQThreads / 32];
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) quant_kernel(const T* __restrict__ x, int64_t ldx, int K, int8_t* __restrict__ q,
+                                                   int64_t ldq, float* __restrict__ sx) {
+  __shared__ uint32_t red[NT / 32];
   pdl_trigger();
   const int tid = threadIdx.x, nc = K / 8;
   const uint4* row = reinterpret_cast<const uint4*>(x + blockIdx.x * ldx);
@@ -103,18 +106,18 @@ __global__ void __launch_bounds__(kQThreads) quant_kernel(const T* __restrict__ 
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kQChunks; ++i) {
-    const int c = tid + i * kQThreads;
+    const int c = tid + i * NT;
     v[i] = c < nc ? row[c] : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < kQChunks; ++i) top = top_bits(v[i], top);
-  for (int c = tid + kQChunks * kQThreads; c < nc; c += kQThreads) top = top_bits(row[c], top);
+  for (int c = tid + kQChunks * NT; c < nc; c += NT) top = top_bits(row[c], top);  // K > 32 * NT: read twice
   top = max(top & 0xffffu, top >> 16);
   top = __reduce_max_sync(0xffffffffu, top);
   if ((tid & 31) == 0) red[tid >> 5] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kQThreads / 32; ++w) top = max(top, red[w]);
+  for (int w = 0; w < NT / 32; ++w) top = max(top, red[w]);
   const float amax = Ty<T>::f2(top).x;
   const bool zero = top == 0, bad = top >= Ty<T>::kInf;
   const float inv = __fdiv_rn(127.f, amax);
@@ -123,11 +126,10 @@ __global__ void __launch_bounds__(kQThreads) quant_kernel(const T* __restrict__ 
   const bool none = zero || bad;
 #pragma unroll
   for (int i = 0; i < kQChunks; ++i) {
-    const int c = tid + i * kQThreads;
+    const int c = tid + i * NT;
     if (c < nc) out[c] = none ? make_uint2(0, 0) : quant8<T>(v[i], inv, amax);
   }
-  for (int c = tid + kQChunks * kQThreads; c < nc; c += kQThreads)
-    out[c] = none ? make_uint2(0, 0) : quant8<T>(row[c], inv, amax);
+  for (int c = tid + kQChunks * NT; c < nc; c += NT) out[c] = none ? make_uint2(0, 0) : quant8<T>(row[c], inv, amax);
 }
 
 // ---------------------------------------------------------------- products
@@ -145,6 +147,7 @@ struct GemmParams {
   int vec;       // rows of c and res start on 16 bytes and hold a multiple of 8 columns
   int m_box;     // small: rows of A that a CTA loads (a multiple of 8)
   int nst;       // small: ring stages
+  int deep;      // small: K blocks per stage (one wait and one commit for 4 * deep MMAs)
   int* err;
 };
 
@@ -198,7 +201,9 @@ HM_DEV void res16(const GemmParams& P, int m, int col, float (&r)[16]) {
 }
 
 // ---------------------------------------------------------------- few tokens: one tile per CTA
-constexpr int kSmallThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
+// Warps: 0 streams W, 1 issues the MMAs, 2 streams A, 3-6 the epilogue.  MT = 64 or 128 rows per MMA
+// (an MMA with 64 rows takes two thirds of the time of one with 128 at BN = 64).
+constexpr int kSmallThreads = 224;
 constexpr int kMaxStages = 16;
 
 struct SmallBars {
@@ -207,112 +212,121 @@ struct SmallBars {
   int abort_flag;
 };
 
-template <int BN, int EPI, typename T>
+template <int BN, int EPI, int MT, typename T>
 __global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_constant__ CUtensorMap amap,
                                                                    const __grid_constant__ CUtensorMap wmap,
                                                                    const __grid_constant__ GemmParams P) {
-  extern __shared__ uint8_t smem_raw[];  // A stages (m_box rows each), then W stages (BN rows each)
+  extern __shared__ uint8_t smem_raw[];  // A stages (deep blocks of m_box rows), then W stages (deep x BN rows)
   uint8_t* const ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ SmallBars sm;
   __shared__ float scl[BN];
-  constexpr uint32_t kCols = BN < 32 ? 32 : BN;
+  constexpr int W = EPI == HM_EPI_SILU ? BN / 2 : BN;  // output columns of the tile
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nt = blockIdx.x, m0 = blockIdx.y * BM;
-  const int nk = (P.K + BK - 1) / BK, nst = P.nst;
-  const uint32_t a_bytes = static_cast<uint32_t>(P.m_box) * BK, w_bytes = BN * BK;
+  const int nst = P.nst, deep = P.deep;
+  const int nb = (P.K + BK - 1) / BK, nk = (nb + deep - 1) / deep;  // K blocks, stages to fill
+  constexpr uint32_t w_block = BN * BK;
+  const uint32_t a_block = static_cast<uint32_t>(P.m_box) * BK, a_bytes = deep * a_block, w_bytes = deep * w_block;
   uint8_t* const wring = ring + nst * a_bytes;
   int* const err = P.err;
   volatile int* abort_s = &sm.abort_flag;
   if (tid == 0) {
     sm.abort_flag = 0;
     for (int i = 0; i < nst; ++i) {
-      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.full[i], 2);  // both producers' expect_tx
       mbar_init(&sm.empty[i], 1);
     }
     mbar_init(&sm.acc_full, 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&sm.tmem_base, kCols);
+  if (warp == 1) tmem_alloc(&sm.tmem_base, BN);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  constexpr int W = EPI == HM_EPI_SILU ? BN / 2 : BN;  // output columns of the tile
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      prefetch_tensormap(&wmap);
-      prefetch_tensormap(&amap);
-      auto load_w = [&](int kb, int s) {
-        mbar_arrive_expect_tx(&sm.full[s], a_bytes + w_bytes);
-        tma_load_2d_plain(wring + s * w_bytes, &wmap, kb * BK, nt * W, &sm.full[s]);
-        if (EPI == HM_EPI_SILU) tma_load_2d_plain(wring + s * w_bytes + W * BK, &wmap, kb * BK, P.w3 + nt * W, &sm.full[s]);
-      };
-      const int pre = min(nk, nst);
-      for (int kb = 0; kb < pre; ++kb) load_w(kb, kb);  // the weights do not depend on the launch before
-      pdl_wait();
-      for (int kb = 0; kb < pre; ++kb) tma_load_2d_plain(ring + kb * a_bytes, &amap, kb * BK, m0, &sm.full[kb]);
-      for (int kb = pre; kb < nk; ++kb) {
-        const int s = kb % nst;
-        if (!mbar_wait_ab(&sm.empty[s], ((kb / nst) - 1) & 1, err, abort_s)) break;
-        load_w(kb, s);
-        tma_load_2d_plain(ring + s * a_bytes, &amap, kb * BK, m0, &sm.full[s]);
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------ TMA producers
+    // the weights do not depend on the launch before, so only the tokens wait for it
+    if (warp == 2) pdl_wait();
+    for (int kb = 0, s = 0, ph = 1; kb < nk; ++kb) {
+      if (kb >= nst && !mbar_wait_short(&sm.empty[s], ph, err, abort_s)) break;
+      if (elect_one()) {
+        const int n = min(deep, nb - kb * deep);  // the last stage may hold fewer blocks
+        if (warp == 0) {
+          mbar_arrive_expect_tx(&sm.full[s], n * w_block);
+          uint8_t* dst = wring + s * w_bytes;
+          for (int d = 0; d < n; ++d, dst += w_block) {
+            tma_load_2d_plain(dst, &wmap, (kb * deep + d) * BK, nt * W, &sm.full[s]);
+            if (EPI == HM_EPI_SILU) tma_load_2d_plain(dst + W * BK, &wmap, (kb * deep + d) * BK, P.w3 + nt * W, &sm.full[s]);
+          }
+        } else {
+          mbar_arrive_expect_tx(&sm.full[s], n * a_block);
+          uint8_t* dst = ring + s * a_bytes;
+          for (int d = 0; d < n; ++d, dst += a_block) tma_load_2d_plain(dst, &amap, (kb * deep + d) * BK, m0, &sm.full[s]);
+        }
+      }
+      __syncwarp();
+      if (++s == nst) {
+        s = 0;
+        ph ^= 1;
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_i8(BM, BN);
-      const uint64_t a0 = sw128_desc(smem_u32(ring)), b0 = sw128_desc(smem_u32(wring));
-      for (int kb = 0; kb < nk; ++kb) {
-        const int s = kb % nst;
-        mbar_wait_ab(&sm.full[s], (kb / nst) & 1, err, abort_s);
-        tc_fence_after();
-        const uint64_t ad = a0 + s * (a_bytes >> 4), bd = b0 + s * (w_bytes >> 4);
+    constexpr uint32_t idesc = idesc_i8(MT, BN);
+    const uint64_t a0 = sw128_desc(smem_u32(ring)), b0 = sw128_desc(smem_u32(wring));
+    for (int kb = 0, s = 0, ph = 0; kb < nk; ++kb) {
+      mbar_wait_short(&sm.full[s], ph, err, abort_s);
+      tc_fence_after();
+      if (elect_one()) {
+        const int n = min(deep, nb - kb * deep);
+        uint64_t ad = a0 + s * (a_bytes >> 4), bd = b0 + s * (w_bytes >> 4);
+        for (int d = 0; d < n; ++d, ad += a_block >> 4, bd += w_block >> 4) {
 #pragma unroll
-        for (int k = 0; k < BK / 32; ++k) umma_i8(tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+          for (int k = 0; k < BK / 32; ++k) umma_i8(tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | d | k) != 0);
+        }
         umma_commit(&sm.empty[s]);
+        if (kb == nk - 1) umma_commit(&sm.acc_full);
       }
-      umma_commit(&sm.acc_full);
+      __syncwarp();
+      if (++s == nst) {
+        s = 0;
+        ph ^= 1;
+      }
     }
   } else {
     // ------------------------------------------------------------ epilogue: a row per thread
-    const int et = tid - 64, quad = warp & 3;  // TMEM lanes 32 * (warp % 4) ..
+    const int et = tid - 96, quad = warp & 3;  // TMEM lanes 32 * (warp % 4) ..
     for (int i = et; i < BN; i += 128) {
       const int col = EPI == HM_EPI_SILU ? nt * W + i % W : nt * W + i;
       scl[i] = col < P.N ? __half2float(P.s[col + (EPI == HM_EPI_SILU && i >= W ? P.w3 : 0)]) : 0.f;
     }
     named_bar(1, 128);
-    const int m = m0 + 32 * quad + lane;
+    // rows of the accumulator: 32 per warp, or (64-row MMA) 16 in the lower lanes of each
+    const int r0 = MT == 64 ? 16 * quad : 32 * quad;
+    const int m = MT == 64 && lane >= 16 ? P.M : m0 + r0 + lane;
     pdl_wait();
     const float sx = m < P.M ? P.sx[m] : 0.f;
-    mbar_wait_ab(&sm.acc_full, 0, err, abort_s);
+    mbar_wait_short(&sm.acc_full, 0, err, abort_s);
     tc_fence_after();
-    if (m0 + 32 * quad < P.M) {  // whole warps (tcgen05.ld is warp-wide)
+    if (m0 + r0 < P.M) {  // whole warps (tcgen05.ld is warp-wide)
       const uint32_t trow = tmem + (static_cast<uint32_t>(32 * quad) << 16);
-      constexpr int STEP = W < 16 ? 8 : 16;
 #pragma unroll 1
-      for (int c0 = 0; c0 < W; c0 += STEP) {
+      for (int c0 = 0; c0 < W; c0 += 16) {
         __syncwarp();  // rows behind the last one skipped the stores
         float y[16];
         if (EPI == HM_EPI_SILU) {
           float a[16], b[16];
-          if (W < 16) {  // BN = 16: columns 0-7 are w1's, 8-15 w3's
-            tmem_ld16(trow, a);
+          tmem_ld16(trow + c0, a);
+          tmem_ld16(trow + W + c0, b);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = a[8 + i];
-          } else {
-            tmem_ld16(trow + c0, a);
-            tmem_ld16(trow + W + c0, b);
-          }
-#pragma unroll
-          for (int i = 0; i < STEP; ++i)
+          for (int i = 0; i < 16; ++i)
             y[i] = silu_f(scaled(a[i], sx, scl[c0 + i])) * scaled(b[i], sx, scl[W + c0 + i]);
         } else {
           tmem_ld16(trow + c0, y);
 #pragma unroll
-          for (int i = 0; i < STEP; ++i) y[i] = scaled(y[i], sx, scl[c0 + i]);
+          for (int i = 0; i < 16; ++i) y[i] = scaled(y[i], sx, scl[c0 + i]);
         }
         const int col = nt * W + c0;
         if (m >= P.M || col >= P.N) continue;
@@ -320,18 +334,18 @@ __global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_
           float r[16];
           res16<T>(P, m, col, r);
 #pragma unroll
-          for (int i = 0; i < STEP; ++i) y[i] += r[i];
+          for (int i = 0; i < 16; ++i) y[i] += r[i];
         }
         T* c = reinterpret_cast<T*>(P.c) + (int64_t)m * P.ldc + col;
-        if (P.vec && col + STEP <= P.N) {
+        if (P.vec && col + 16 <= P.N) {
 #pragma unroll
-          for (int h = 0; h < STEP / 8; ++h)
+          for (int h = 0; h < 2; ++h)
             reinterpret_cast<uint4*>(c)[h] =
                 make_uint4(Ty<T>::pack(y[8 * h], y[8 * h + 1]), Ty<T>::pack(y[8 * h + 2], y[8 * h + 3]),
                            Ty<T>::pack(y[8 * h + 4], y[8 * h + 5]), Ty<T>::pack(y[8 * h + 6], y[8 * h + 7]));
         } else {
 #pragma unroll
-          for (int i = 0; i < STEP; ++i)
+          for (int i = 0; i < 16; ++i)
             if (col + i < P.N) c[i] = Ty<T>::one(y[i]);
         }
       }
@@ -341,7 +355,7 @@ __global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, kCols);
+    tmem_dealloc(tmem, BN);
   }
 }
 
@@ -471,24 +485,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       prefetch_tensormap(&amap);
       prefetch_tensormap(&wmap);
-      const uint32_t full0 = dsmem_addr(&sm.full[0], 0);
-      int g = 0;
-      for (int t = pair; t < tiles; t += npairs) {
-        const int mp = P.n_fast ? t / P.ntiles : t % mpairs, nt = P.n_fast ? t % P.ntiles : t / mpairs;
-        const int m_row0 = mp * 2 * BM + static_cast<int>(rank) * BM;
-        const int brow = EPI == HM_EPI_SILU ? (rank == 0 ? 0 : P.w3) + nt * WT : nt * WT + static_cast<int>(rank) * BM;
-        for (int kb = 0; kb < nk; ++kb, ++g) {
-          const int s = g % NS2;
-          if (g >= NS2) mbar_wait_ab(&sm.empty[s], ((g / NS2) - 1) & 1, err, abort_s);
+    }
+    __syncwarp();
+    const uint32_t full0 = dsmem_addr(&sm.full[0], 0);
+    int g = 0;
+    for (int t = pair; t < tiles; t += npairs) {
+      const int mp = P.n_fast ? t / P.ntiles : t % mpairs, nt = P.n_fast ? t % P.ntiles : t / mpairs;
+      const int m_row0 = mp * 2 * BM + static_cast<int>(rank) * BM;
+      const int brow = EPI == HM_EPI_SILU ? (rank == 0 ? 0 : P.w3) + nt * WT : nt * WT + static_cast<int>(rank) * BM;
+      for (int kb = 0; kb < nk; ++kb, ++g) {
+        const int s = g % NS2;
+        if (g >= NS2) mbar_wait_short(&sm.empty[s], ((g / NS2) - 1) & 1, err, abort_s);
+        if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kTileBytes);
           tma_load_2d_pair(sm.a[s], &amap, kb * BK, m_row0, full0 + 8 * s);
           tma_load_2d_pair(sm.b[s], &wmap, kb * BK, brow, full0 + 8 * s);
         }
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader CTA)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_i8(2 * BM, BN2);
       const uint64_t a0 = sw128_desc(smem_u32(sm.a[0])), b0 = sw128_desc(smem_u32(sm.b[0]));
       int g = 0, i = 0;
@@ -499,14 +517,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t acc = tmem + ab * BN2;
         for (int kb = 0; kb < nk; ++kb, ++g) {
           const int s = g % NS2;
-          mbar_wait_ab(&sm.full[s], (g / NS2) & 1, err, abort_s);
+          mbar_wait_short(&sm.full[s], (g / NS2) & 1, err, abort_s);
           tc_fence_after();
-          const uint64_t ad = a0 + s * (kTileBytes >> 4), bd = b0 + s * (kTileBytes >> 4);
+          if (elect_one()) {
+            const uint64_t ad = a0 + s * (kTileBytes >> 4), bd = b0 + s * (kTileBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) umma_i8_pair(acc, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
-          umma_commit_pair(&sm.empty[s]);
+            for (int k = 0; k < BK / 32; ++k) umma_i8_pair(acc, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+            umma_commit_pair(&sm.empty[s]);
+            if (kb == nk - 1) umma_commit_pair(&sm.acc_full[ab]);
+          }
+          __syncwarp();
         }
-        umma_commit_pair(&sm.acc_full[ab]);
       }
     }
   } else {
@@ -517,7 +538,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int ab = i & 1;
       const int mp = P.n_fast ? t / P.ntiles : t % mpairs, nt = P.n_fast ? t % P.ntiles : t / mpairs;
       const int m_row0 = mp * 2 * BM + static_cast<int>(rank) * BM;
-      mbar_wait_ab(&sm.acc_full[ab], (i >> 1) & 1, err, abort_s);
+      mbar_wait_short(&sm.acc_full[ab], (i >> 1) & 1, err, abort_s);
       tc_fence_after();
       pair_epilogue<EPI, T>(P, tmem + ab * BN2, warp, lane, m_row0, nt, sm.stage, sm.scl[ab], [&] {
         tc_fence_before();
@@ -573,22 +594,40 @@ cudaError_t max_smem(K kernel, std::atomic<bool>* configured, int dev, size_t by
   return e;
 }
 
-constexpr int kSmallRing = 106 * 1024;  // a small CTA's ring: two CTAs per SM
+// A small CTA's ring: two CTAs per SM, or one when the grid has no more CTAs than SMs.
+constexpr int kRingTwo = 106 * 1024, kRingOne = 200 * 1024;
 
-template <int BN, int EPI, typename T>
-cudaError_t launch_small(const CUtensorMap& am, const CUtensorMap& wm, GemmParams p, int dev, int pdl, cudaStream_t st) {
+template <int BN, int EPI, int MT, typename T>
+cudaError_t launch_small(const CUtensorMap& am, const CUtensorMap& wm, GemmParams p, int sms, int dev, int pdl,
+                         cudaStream_t st) {
   static std::atomic<bool> configured[kMaxDevices];
-  cudaError_t e = max_smem(gemm_small_kernel<BN, EPI, T>, configured, dev, kSmallRing + 1024);
+  const cudaError_t e = max_smem(gemm_small_kernel<BN, EPI, MT, T>, configured, dev, kRingOne + 1024);
   if (e != cudaSuccess) return e;
-  const int stage = (p.m_box + BN) * BK, nk = (p.K + BK - 1) / BK;
-  p.nst = kSmallRing / stage < kMaxStages ? kSmallRing / stage : kMaxStages;
-  if (p.nst > nk) p.nst = nk;
-  // at the last A stage the MMA reads 128 rows: they have to lie inside the allocation
-  const int reach = (p.nst - 1) * p.m_box * BK + BM * BK, ring = p.nst * stage > reach ? p.nst * stage : reach;
-  static_assert(kSmallRing / ((BM + 128) * BK) >= 3 && 2 * kSmallRing + 6 * 1024 <= 228 * 1024, "ring");
   constexpr int W = EPI == HM_EPI_SILU ? BN / 2 : BN;
   const dim3 grid((p.N + W - 1) / W, (p.M + BM - 1) / BM);
-  return hm_launch(gemm_small_kernel<BN, EPI, T>, grid, dim3(kSmallThreads), static_cast<size_t>(ring) + 1024, st, pdl, am, wm, p);
+  const int room = (int64_t)grid.x * grid.y <= sms ? kRingOne : kRingTwo;
+  const int block = (p.m_box + BN) * BK, nb = (p.K + BK - 1) / BK;
+  p.deep = 4;
+  while (p.deep > 1 && room / (p.deep * block) < 3) p.deep /= 2;
+  const int nk = (nb + p.deep - 1) / p.deep;
+  p.nst = room / (p.deep * block) < kMaxStages ? room / (p.deep * block) : kMaxStages;
+  if (p.nst > nk) p.nst = nk;
+  static_assert(kRingTwo / ((MT + BN) * BK) >= 3 && 2 * kRingTwo + 6 * 1024 <= 228 * 1024 && kRingOne + 3 * 1024 <= 227 * 1024,
+                "ring");
+  // from the last A block the MMA reads MT rows: they have to lie inside the allocation
+  const int used = p.nst * p.deep * block, reach = (p.deep * p.nst - 1) * p.m_box * BK + MT * BK;
+  return hm_launch(gemm_small_kernel<BN, EPI, MT, T>, grid, dim3(kSmallThreads),
+                   static_cast<size_t>(used > reach ? used : reach) + 1024, st, pdl, am, wm, p);
+}
+
+template <int EPI, int MT, typename T>
+cudaError_t launch_bn(const CUtensorMap& am, const CUtensorMap& wm, const GemmParams& p, int bn, int sms, int dev,
+                      int pdl, cudaStream_t st) {
+  switch (bn) {
+    case 128: return launch_small<128, EPI, MT, T>(am, wm, p, sms, dev, pdl, st);
+    case 64: return launch_small<64, EPI, MT, T>(am, wm, p, sms, dev, pdl, st);
+    default: return launch_small<32, EPI, MT, T>(am, wm, p, sms, dev, pdl, st);
+  }
 }
 
 template <int EPI, typename T>
@@ -619,25 +658,24 @@ cudaError_t launch_gemm(const int8_t* q, int64_t ldq, const int8_t* w, GemmParam
   }
   const int mt = (p.M + BM - 1) / BM;
   p.m_box = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
-  // the widest tile whose grid takes the fewest columns per SM
-  int bn = 128;
+  // the tile width whose CTAs cost an SM the least: cycles per MMA (measured, with a share of the
+  // waits) times the CTAs that an SM gets.  1 x 5120 x 4096: 8.2 us at 64, 8.9 at 32, 10.1 at 128.
+  const int64_t cycles[2][3] = {{37, 45, 77}, {53, 61, 77}};
+  int bn = 0;
   int64_t best = INT64_MAX;
-  for (int b = 128; b >= 16; b /= 2) {
-    const int64_t tiles = (int64_t)mt * ((wrows + b - 1) / b), cost = (tiles + sms - 1) / sms * b;
+  for (int i = 2; i >= 0; --i) {
+    const int64_t tiles = (int64_t)mt * ((wrows + (32 << i) - 1) / (32 << i));
+    const int64_t cost = (tiles + sms - 1) / sms * cycles[p.M > 64][i];
     if (cost < best) {
       best = cost;
-      bn = b;
+      bn = 32 << i;
     }
   }
   if (!tile_map(q, p.M, p.K, ldq, p.m_box, &am) ||
       !tile_map(w, wrows, p.K, p.K, EPI == HM_EPI_SILU ? bn / 2 : bn, &wm))
     return cudaErrorInvalidValue;
-  switch (bn) {
-    case 128: return launch_small<128, EPI, T>(am, wm, p, dev, pdl, st);
-    case 64: return launch_small<64, EPI, T>(am, wm, p, dev, pdl, st);
-    case 32: return launch_small<32, EPI, T>(am, wm, p, dev, pdl, st);
-    default: return launch_small<16, EPI, T>(am, wm, p, dev, pdl, st);
-  }
+  return p.M <= 64 ? launch_bn<EPI, 64, T>(am, wm, p, bn, sms, dev, pdl, st)
+                   : launch_bn<EPI, 128, T>(am, wm, p, bn, sms, dev, pdl, st);
 }
 
 bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u); }
@@ -658,7 +696,11 @@ bool out_ok(const int8_t* w, const void* s, const void* res, int64_t ldr, const 
 
 template <typename T>
 cudaError_t quantise(const void* x, int64_t ldx, int M, int K, int8_t* q, int64_t ldq, float* sx, cudaStream_t st) {
-  return hm_launch(quant_kernel<T>, dim3(M), dim3(kQThreads), 0, st, 0, reinterpret_cast<const T*>(x), ldx, K, q, ldq, sx);
+  const T* p = reinterpret_cast<const T*>(x);
+  // as few threads as keep a row in registers: more rows in flight per SM
+  if (K <= 128 * 8 * kQChunks) return hm_launch(quant_kernel<T, 128>, dim3(M), dim3(128), 0, st, 0, p, ldx, K, q, ldq, sx);
+  if (K <= 256 * 8 * kQChunks) return hm_launch(quant_kernel<T, 256>, dim3(M), dim3(256), 0, st, 0, p, ldx, K, q, ldq, sx);
+  return hm_launch(quant_kernel<T, 512>, dim3(M), dim3(512), 0, st, 0, p, ldx, K, q, ldq, sx);
 }
 
 cudaError_t multiply(const int8_t* q, int64_t ldq, const float* sx, int dtype, const int8_t* w, const void* s,

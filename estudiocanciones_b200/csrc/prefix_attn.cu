@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
           const int st = it % NST;
           const uint32_t no = __ballot_sync(0xffffffffu, bad) >> (i * nsub);
           int ok = 1;
-          if (lane == 0 && it >= NST) ok = mbar_wait_ab(&sm.empty[st], ((it / NST) - 1) & 1, P.err, &sm.abort_flag);
+          if (lane == 0 && it >= NST) ok = mbar_wait_short(&sm.empty[st], ((it / NST) - 1) & 1, P.err, &sm.abort_flag);
           go = __shfl_sync(0xffffffffu, ok, 0);
           if (!go) break;
           if (lane == 0) {
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       const int first = J.lo / kTile;
       for (int tt = r.t0; tt < r.t1; ++tt, ++it) {
         const int st = it % NST;
-        mbar_wait_ab(&sm.full[st], (it / NST) & 1, P.err, &sm.abort_flag);  // on timeout: carry on, error flagged
+        mbar_wait_short(&sm.full[st], (it / NST) & 1, P.err, &sm.abort_flag);  // on timeout: carry on, error flagged
         const int bad = sm.bad[st], p0 = (first + tt) * kTile;
         if (J.big)
           C.template tile<4>(st, p0, J, bad);

@@ -36,6 +36,7 @@ There is no CPU fallback: non-CUDA tensors raise.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -288,6 +289,12 @@ def _launch(idx: int, what: str, *args) -> None:
         check(rc, what)
 
 
+@functools.lru_cache(maxsize=4096)
+def _size(what: str, *args) -> int:
+    """A size function of the library (a function of its arguments alone)."""
+    return getattr(_lib.lib(), what)(*args)
+
+
 # ----------------------------------------------------------------------------- pages of a KV cache
 MAX_LIST = 1024   # sequences or pages of one call
 
@@ -319,23 +326,26 @@ def _page_state(what: str, table, lens, refs, page: int):
     if lens is not None and (lens.dtype != torch.int64 or lens.dim() != 1 or lens.numel() != n or
                              not lens.is_contiguous()):
         raise HMError(f"{what}: lens is int64 [sequences]")
-    if refs.dtype != torch.int32 or refs.dim() != 1 or refs.numel() < 1 or not refs.is_contiguous():
+    n_pages = refs.numel()
+    if refs.dtype != torch.int32 or refs.dim() != 1 or n_pages < 1 or not refs.is_contiguous():
         raise HMError(f"{what}: refs is int32 [pages of the pool]")
     if not 1 <= page <= 1024:
         raise HMError(f"{what}: a page holds 1 to 1024 positions")
-    return idx, _lib.PageState(table.data_ptr(), table.stride(0), None if lens is None else lens.data_ptr(),
-                               refs.data_ptr(), _err_ptr(idx), n, mp, refs.numel(), page)
+    return idx, _lib.PACK_PAGE_STATE.pack(table.data_ptr(), table.stride(0), 0 if lens is None else lens.data_ptr(),
+                                          refs.data_ptr(), _err_ptr(idx), n, mp, n_pages, page)
 
 
 def _page_pool(what: str, k, v):
-    if (k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous() or
+    """(hm_page_pool, pages of the pool, positions of a page)."""
+    shape = k.shape
+    if (len(shape) != 5 or v.shape != shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous() or
             k.numel() == 0):
         raise HMError(f"{what}: k and v are contiguous [layers, pages, Hk, page, hd] of one type")
-    layers, n_pages, hk, page, hd = k.shape
+    layers, n_pages, hk, page, hd = shape
     row = hd * k.element_size()
     if row % 16:
         raise HMError(f"{what}: a position of a head is a multiple of 16 bytes")
-    return _lib.PagePoolDesc(k.data_ptr(), v.data_ptr(), layers, n_pages, hk, page, row)
+    return _lib.PACK_PAGE_POOL.pack(k.data_ptr(), v.data_ptr(), layers, n_pages, hk, page, row), n_pages, page
 
 
 def pages_grow(table, lens, refs, page: int, seqs, n: int = 1) -> None:
@@ -362,7 +372,7 @@ def pages_free(table, lens, refs, seqs) -> None:
 
 def _moves(what: str, n_moves: int, n_pages: int, like):
     """Scratch of a call that moves pages: (tensor, bytes)."""
-    nbytes = _lib.lib().hm_pages_workspace_bytes(n_moves, n_pages)
+    nbytes = _size("hm_pages_workspace_bytes", n_moves, n_pages)
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes
 
 
@@ -370,9 +380,9 @@ def pages_fork(k, v, table, lens, refs, src, dst) -> None:
     """Empty sequence ``dst[i]`` becomes a copy of sequence ``src[i]``: full pages are shared, the
     positions of a partial last page are copied (every layer, K and V) into a free page."""
     _device_of("pages_fork", table, k, v)
-    pool = _page_pool("pages_fork", k, v)
-    idx, st = _page_state("pages_fork", table, lens, refs, pool.page)
-    if refs.numel() != pool.n_pages:
+    pool, n_pages, page = _page_pool("pages_fork", k, v)
+    idx, st = _page_state("pages_fork", table, lens, refs, page)
+    if refs.numel() != n_pages:
         raise HMError("pages_fork: refs has one count per page of the pool")
     src, dst = _ids("pages_fork", src, table), _ids("pages_fork", dst, table)
     n = dst.numel()
@@ -386,7 +396,7 @@ def pages_copy(k, v, src, dst) -> None:
     """Pages ``dst[i]`` become copies of pages ``src[i]`` in every layer, K and V.  No page may be a
     target twice, or a target and a source."""
     idx = _device_of("pages_copy", k, v)
-    pool = _page_pool("pages_copy", k, v)
+    pool = _page_pool("pages_copy", k, v)[0]
     src, dst = _ids("pages_copy", src, k), _ids("pages_copy", dst, k)
     n = dst.numel()
     if src.numel() != n:
@@ -400,19 +410,20 @@ def pages_compact(k, v, table, refs) -> torch.Tensor:
     move into the free ones below it, in ascending order, and the table follows.  Returns the
     count, int32 ``[1]`` on the device."""
     _device_of("pages_compact", table, k, v)
-    pool = _page_pool("pages_compact", k, v)
-    idx, st = _page_state("pages_compact", table, None, refs, pool.page)
-    if refs.numel() != pool.n_pages:
+    pool, n_pages, page = _page_pool("pages_compact", k, v)
+    idx, st = _page_state("pages_compact", table, None, refs, page)
+    if refs.numel() != n_pages:
         raise HMError("pages_compact: refs has one count per page of the pool")
     n_live = torch.empty(1, dtype=torch.int32, device=table.device)
-    ws, nbytes = _moves("pages_compact", pool.n_pages // 2, pool.n_pages, table)
+    ws, nbytes = _moves("pages_compact", n_pages // 2, n_pages, table)
     _launch(idx, "hm_pages_compact", st, pool, n_live.data_ptr(), ws.data_ptr(), nbytes)
     return n_live
 
 
-def _layer_pages(what: str, k, v, table, seqs, R: int, S: int) -> None:
-    """One layer's pool and the rows of its table that R query rows use."""
-    if (k.dtype not in _DT or k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or
+def _layer_pages(what: str, k, v, table, seqs, R: int, S: int):
+    """One layer's pool and the rows of its table that R query rows use; returns the pool's shape."""
+    shape, dt = k.shape, k.dtype
+    if (dt not in _DT or len(shape) != 4 or v.shape != shape or v.dtype != dt or not k.is_contiguous() or
             not v.is_contiguous() or k.numel() == 0):
         raise HMError(f"{what}: k and v are contiguous fp16 or bf16 [pages, Hk, page, hd]")
     if not _is_table(table):
@@ -424,6 +435,7 @@ def _layer_pages(what: str, k, v, table, seqs, R: int, S: int) -> None:
             raise HMError(f"{what}: the table has a row for every sequence")
     elif seqs.dtype != torch.int32 or seqs.shape != (R // S,) or not seqs.is_contiguous():
         raise HMError(f"{what}: seqs is int32 [sequences]")
+    return shape
 
 
 def _is_rows(t, R: int, W: int) -> bool:
@@ -437,8 +449,7 @@ def rope_pages(qkv, rope, pos, q_out, k, v, table, S: int, Hq: int, Hk: int, seq
     A padding row has ``pos[r] < 0``: its ``q_out`` is zero and nothing is written."""
     idx = _device_of("rope_pages", qkv, rope, pos, q_out, k, v, table, seqs)
     R = qkv.shape[0]
-    _layer_pages("rope_pages", k, v, table, seqs, R, S)
-    n_pages, hk, page, hd = k.shape
+    n_pages, hk, page, hd = _layer_pages("rope_pages", k, v, table, seqs, R, S)
     if hk != Hk or hd % 8:
         raise HMError("rope_pages: Hk heads of a multiple of 8 dims")
     if qkv.dtype != k.dtype or q_out.dtype != k.dtype or not _is_rows(qkv, R, (Hq + 2 * Hk) * hd):
@@ -482,37 +493,40 @@ def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int 
     if q.dim() != 2:
         raise HMError("prefix_attn: q [R, Hq * hd]")
     R, W = q.shape
-    _layer_pages("prefix_attn", k, v, table, seqs, R, S)
-    n_pages, Hk, page, hd = k.shape
-    Hq = W // hd
-    if q.dtype != k.dtype or W != Hq * hd or Hq < Hk or Hq % Hk or q.stride(1) != 1:
+    n_pages, Hk, page, hd = _layer_pages("prefix_attn", k, v, table, seqs, R, S)
+    Hq, dt = W // hd, q.dtype
+    if dt != k.dtype or W != Hq * hd or Hq < Hk or Hq % Hk or q.stride(1) != 1:
         raise HMError("prefix_attn: q [R, Hq * hd] of the cache's type, Hq a multiple of Hk")
     if o is None:
-        o = torch.empty(R, W, dtype=q.dtype, device=q.device)
-    elif o.dtype != q.dtype or not _is_rows(o, R, W):
+        o = torch.empty((R, W), dtype=dt, device=q.device)
+    elif o.dtype != dt or not _is_rows(o, R, W):
         raise HMError("prefix_attn: o is like q")
     if pos.dtype != torch.int64 or pos.dim() != 1 or pos.numel() != R or not pos.is_contiguous():
         raise HMError("prefix_attn: pos is int64 [R]")
-    groups = 0
+    groups = gs = ow = pl = 0
     if gstart is not None:
         groups = gstart.numel() - 1
         if owner is None or plen is None:
             raise HMError("prefix_attn: gstart comes with owner and plen")
-        for t, n in ((gstart, groups + 1), (owner, groups), (plen, groups)):
-            if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or n < 0 or not t.is_contiguous():
-                raise HMError("prefix_attn: gstart [groups + 1], owner and plen [groups] are int32 vectors")
+        i32 = torch.int32
+        if (groups < 0 or gstart.dtype != i32 or owner.dtype != i32 or plen.dtype != i32 or gstart.dim() != 1 or
+                owner.shape != (groups,) or plen.shape != (groups,) or not gstart.is_contiguous() or
+                not owner.is_contiguous() or not plen.is_contiguous()):
+            raise HMError("prefix_attn: gstart [groups + 1], owner and plen [groups] are int32 vectors")
+        if groups:
+            gs, ow, pl = gstart.data_ptr(), owner.data_ptr(), plen.data_ptr()
     elif owner is not None or plen is not None:
         raise HMError("prefix_attn: owner and plen come with gstart")
-    nbytes = _lib.lib().hm_prefix_attn_workspace_bytes(R, S, Hq, Hk, hd, groups, _sms(idx))
+    nbytes = _size("hm_prefix_attn_workspace_bytes", R, S, Hq, Hk, hd, groups, _sms(idx))
     if nbytes == 0:
         raise HMError("prefix_attn: hd 64, 128 or 256, up to 64 query heads per KV head and 1024 row blocks")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    d = _lib.PrefixAttnDesc(q.data_ptr(), q.stride(0) if R > 1 else W, o.data_ptr(), o.stride(0) if R > 1 else W,
-                            k.data_ptr(), v.data_ptr(), pos.data_ptr(), table.data_ptr(), table.stride(0),
-                            None if seqs is None else seqs.data_ptr(), gstart.data_ptr() if groups > 0 else None,
-                            owner.data_ptr() if groups > 0 else None, plen.data_ptr() if groups > 0 else None,
-                            ws.data_ptr(), nbytes, _err_ptr(idx), _DT[k.dtype], R, S, Hq, Hk, hd, table.shape[0],
-                            table.shape[1], n_pages, page, groups, 1.0 / math.sqrt(hd) if scale is None else scale)
+    n_table, max_pages = table.shape
+    d = _lib.PACK_PREFIX_ATTN.pack(q.data_ptr(), q.stride(0) if R > 1 else W, o.data_ptr(), o.stride(0) if R > 1 else W,
+                                   k.data_ptr(), v.data_ptr(), pos.data_ptr(), table.data_ptr(), table.stride(0),
+                                   0 if seqs is None else seqs.data_ptr(), gs, ow, pl, ws.data_ptr(), nbytes,
+                                   _err_ptr(idx), _DT[dt], R, S, Hq, Hk, hd, n_table, max_pages, n_pages, page, groups,
+                                   1.0 / math.sqrt(hd) if scale is None else scale)
     _launch(idx, "hm_prefix_attn", d)
     return o
 
@@ -599,7 +613,7 @@ def int8_mm_a8(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, res: torch.Ten
     x = _rows16("int8_mm_a8", x)
     M, K = x.shape
     N, out = _a8_out("int8_mm_a8", x.dtype, w, s, res, out, silu, M, K, x.device)
-    nbytes = _lib.lib().hm_int8_mm_a8_workspace_bytes(M, K)
+    nbytes = _size("hm_int8_mm_a8_workspace_bytes", M, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _launch(idx, "hm_int8_mm_a8", x.data_ptr(), _pitch(x), _DT[x.dtype], w.data_ptr(), s.data_ptr(),
             None if res is None else res.data_ptr(), 0 if res is None else _pitch(res), out.data_ptr(), _pitch(out), M,

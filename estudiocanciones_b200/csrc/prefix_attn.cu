@@ -12,17 +12,17 @@
 // position, against 4 * Hq * hd operations a (row, position).  Up to ~100 query rows per KV head
 // that is less than the tensor cores do while the bytes arrive, so the kernel is built to keep
 // the memory busy:
-//  * The work is a list of jobs (group prefix or one sequence's own positions, cut into blocks
+//  * The work is a list of jobs (one sequence's own positions or a group's prefix, cut into blocks
 //    of query rows) x KV heads x tiles of 64 positions.  Lengths live on the device, so every CTA
 //    builds the list itself (one pass over pos, a scan in shared memory) and takes an equal share
-//    of the tiles: a long prefix next to short sequences leaves no SM idle, whatever the lengths.
+//    of the cost: a long prefix next to short sequences leaves no SM idle, whatever the lengths.
 //  * One producer warp fetches page numbers 32 at a time and issues one TMA box per page and
 //    operand (128-byte swizzle) into a ring of 96 KB per CTA, two CTAs per SM, across job
-//    boundaries, so the ring never drains.
-//  * Four consumer warps.  Blocks of up to 16 query rows (the G heads of a KV head x rows): each
-//    warp takes 16 of the tile's positions, so K and V leave shared memory once; the four
-//    partial results meet in shared memory.  Blocks of up to 64 rows: each warp takes 16 rows and
-//    all positions, K and V leave shared memory four times but HBM / L2 only once per 64 rows.
+//    boundaries, so the ring never drains.  It also works out what each run of tiles belongs to
+//    and hands that over with the run's first tile.
+//  * Four consumer warps share a block of query rows (the G heads of a KV head x rows) as
+//    row groups x position groups: 16 rows: 1 x 4 (K and V leave shared memory once), 32 rows:
+//    2 x 2, 64 rows: 4 x 1.  Position groups meet in shared memory at the end of a run.
 //  * A second small kernel joins the partial results of a row in a fixed order (results do not
 //    depend on scheduling) and writes o; its launch overlaps the first kernel's tail.
 // Scores, m, l and a are fp32; the probabilities are rounded to the cache's type for the product
@@ -39,6 +39,8 @@ namespace {
 
 constexpr int kTile = 64;       // positions per tile
 constexpr int kMaxJobs = 1024;  // jobs of a call (the list lives in shared memory)
+constexpr int kMaxPre = 896;    // prefix jobs, and groups, of a call
+constexpr int kMaxRows = 16384; // query rows of a call
 constexpr int kThreads = 160;   // 4 consumer warps + the producer
 constexpr int kCons = 128;
 
@@ -57,20 +59,21 @@ struct Params {
   int R, S, B, Hq, Hk, G, n_table, max_pages, n_pages, page, n_groups;
   int sub_shift;      // log2 of the positions per TMA box (at most a page, at most a tile)
   float scale;        // scale * log2(e)
+  int n_jobs;         // own jobs, then room for the prefix jobs
   int own_blocks;     // row blocks of one sequence's own job
   int own_rows;       // row capacity of an own partial
   int pre_rows;       // row capacity of a prefix partial
   int64_t pre_slots;  // prefix partials come first
-  int* plan;          // header, tile scan, first prefix job of every group (for the join)
+  int* plan;          // what the join needs of the job list
   float* pm;          // [rows] maxima, [rows] sums, [rows][hd] accumulators
   float* pl;
   float* pa;
   int* err;
 };
 
-// plan: 0 prefix jobs, 1 jobs, 2 tiles per CTA, 3 groups unusable; then kMaxJobs + 1 tile offsets;
-// then n_groups first jobs
-constexpr int kPlanScan = 4, kPlanGroup = 4 + kMaxJobs + 1;
+// plan: 0 a CTA's share of the cost, 1 groups unusable; then the cost before every job
+constexpr int kPlanScan = 2, kPlanInts = 2 + kMaxJobs + 1;
+#define HM_HD __host__ __device__ __forceinline__
 
 // ---------------------------------------------------------------- types
 template <typename T>
@@ -96,6 +99,20 @@ struct Ty<__nv_bfloat16> {
   }
 };
 
+// Barrier over the first `n` threads of the CTA that returns whether any of them passed true.
+HM_DEV bool named_bar_or(int id, int n, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"(static_cast<uint32_t>(p))
+      : "memory");
+  return r != 0;
+}
+
 HM_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -103,15 +120,18 @@ HM_DEV float ex2(float x) {
 }
 
 // ---------------------------------------------------------------- lengths and groups
-// Block size of a job with `rows` query rows per KV head: 16 rows while they fit one block.
-HM_DEV int block_rows(int rows) { return rows <= 16 ? 16 : 64; }
+// Block size of a job with `rows` query rows per KV head.
+HM_HD int block_rows(int rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
+// What a tile costs a CTA: up to 32 rows its bytes (about 2800 cycles at an even share of HBM, the
+// arithmetic takes 1600 or 2300), with 64 rows the arithmetic (4200).
+HM_HD int tile_cost(int mt) { return mt <= 32 ? 2 : 3; }
 
 // Positions that row r attends to: 0 for a padding row and for one whose position or table row
 // is out of range (reported).
 HM_DEV int row_len(const Params& P, int r) {
   const int64_t p = P.pos[r];
-  if (p < 0) return 0;
   const int b = r / P.S, s = P.seqs ? P.seqs[b] : b;
+  if (p < 0) return 0;
   if (p >= (int64_t)P.max_pages * P.page || s < 0 || s >= P.n_table) {
     report_error(P.err, HM_ERR_BADINDEX);
     return 0;
@@ -121,9 +141,8 @@ HM_DEV int row_len(const Params& P, int r) {
 
 // Prefix length of a group: 0 when its entry is out of range (reported).
 HM_DEV int group_plen(const Params& P, int g) {
-  const int n = P.plen[g];
+  const int n = P.plen[g], own = P.owner[g];
   if (n == 0) return 0;
-  const int own = P.owner[g];
   if (n < 0 || n > (int64_t)P.max_pages * P.page || own < 0 || own >= P.n_table) {
     report_error(P.err, HM_ERR_BADINDEX);
     return 0;
@@ -131,70 +150,56 @@ HM_DEV int group_plen(const Params& P, int g) {
   return n;
 }
 
-// The group of sequence b (gstart ascending, checked), -1 for none.
-HM_DEV int group_of(const Params& P, int b) {
-  int lo = 0, hi = P.n_groups;  // the first boundary above b
+// The group of sequence b (gs: ascending boundaries), -1 for none.
+HM_DEV int group_of(const int* gs, int n_groups, int b) {
+  int lo = 0, hi = n_groups;  // the first boundary above b
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (P.gstart[mid + 1] <= b)
+    if (gs[mid + 1] <= b)
       lo = mid + 1;
     else
       hi = mid;
   }
-  return lo < P.n_groups && P.gstart[lo] <= b ? lo : -1;
-}
-
-HM_DEV bool bad_boundary(const Params& P, int g) {
-  const int a = P.gstart[g], b = P.gstart[g + 1];
-  return a < 0 || a > b || b > P.B;
+  return lo < n_groups && gs[lo] <= b ? lo : -1;
 }
 
 // One job: query rows i0 .. i0 + M - 1 of `row0` (i -> row row0 + i / G, head kh * G + i % G) over
-// the positions [lo, hi) of table row `trow`.
+// the positions [lo, hi) of table row `trow`.  mt: rows of the block.
 struct Job {
-  int row0, i0, M, lo, hi, trow, big;
+  int row0, i0, M, lo, hi, trow, mt;
 };
 
-HM_DEV Job job_of(const Params& P, int n_pre, const int* ids, int j, bool no_groups) {
+// The first prefix job of a group whose sequences start at a: a group of n rows has at most
+// n / 64 + 1 jobs, so these numbers leave room for all of them without a scan.
+HM_DEV int group_job(const Params& P, int n_own, int g, int a) { return n_own + ((a * P.S * P.G) >> 6) + g; }
+
+// Block blk of group g's prefix (sequences a .. b - 1), and of sequence b's own positions behind a
+// prefix of lo.  hi is not yet cut to what the rows see.
+HM_DEV Job prefix_job(const Params& P, int blk, int a, int b, int plen) {
   Job J;
-  if (j < n_pre) {
-    const int g = ids[j] & 0xffff, blk = ids[j] >> 16;
-    const int a = P.gstart[g];
-    const int rows = (P.gstart[g + 1] - a) * P.S * P.G, mt = block_rows(rows);
-    J.row0 = a * P.S;
-    J.i0 = blk * mt;
-    J.M = min(mt, rows - J.i0);
-    J.big = mt > 16;
-    J.lo = 0;
-    J.hi = P.plen[g];  // in range: groups with a bad entry have no job
-    J.trow = P.owner[g];
-  } else {
-    const int u = j - n_pre, b = u / P.own_blocks, blk = u % P.own_blocks;
-    const int rows = P.S * P.G, mt = block_rows(rows);
-    J.row0 = b * P.S;
-    J.i0 = blk * mt;
-    J.M = min(mt, rows - J.i0);
-    J.big = mt > 16;
-    const int g = no_groups ? -1 : group_of(P, b);
-    J.lo = g < 0 ? 0 : group_plen(P, g);
-    J.hi = (int64_t)P.max_pages * P.page;
-    J.trow = P.seqs ? P.seqs[b] : b;
-  }
+  const int rows = (b - a) * P.S * P.G;
+  J.row0 = a * P.S;
+  J.lo = 0;
+  J.hi = plen;
+  J.mt = block_rows(rows);
+  J.i0 = blk * J.mt;
+  J.M = min(J.mt, rows - J.i0);
+  return J;
+}
+HM_DEV Job own_job(const Params& P, int blk, int b, int lo) {
+  Job J;
+  const int rows = P.S * P.G;
+  J.row0 = b * P.S;
+  J.lo = lo;
+  J.hi = P.max_pages * P.page;
+  J.mt = block_rows(rows);
+  J.i0 = blk * J.mt;
+  J.M = min(J.mt, rows - J.i0);
   return J;
 }
 // First and last query row of a job.
 HM_DEV int row_first(const Params& P, const Job& J) { return J.row0 + J.i0 / P.G; }
 HM_DEV int row_last(const Params& P, const Job& J) { return J.row0 + (J.i0 + J.M - 1) / P.G; }
-
-// The job with hi cut to what its rows see.  Whole warps.
-HM_DEV Job warp_job(const Params& P, int n_pre, const int* ids, int j, bool no_groups) {
-  Job J = job_of(P, n_pre, ids, j, no_groups);
-  int top = 0;
-  for (int r = row_first(P, J) + (threadIdx.x & 31); r <= row_last(P, J); r += 32) top = max(top, row_len(P, r));
-  J.hi = min(J.hi, __reduce_max_sync(0xffffffffu, top));
-  return J;
-}
-
 HM_DEV int tiles_of(const Job& J) { return J.hi > J.lo ? (J.hi - 1) / kTile - J.lo / kTile + 1 : 0; }
 
 // ---------------------------------------------------------------- shared memory
@@ -207,79 +212,104 @@ struct Cfg {
   static constexpr int kQPitch = HD * 2 + 16;
 };
 
+// A run of tiles of one (job, KV head), as the producer hands it to the consumers.
+struct Run {
+  Job J;
+  int kh, tile, tiles;  // first tile (of the cache), their number
+  int slot, prefix;     // number of the partial result among those of its kind
+};
+// Entries of the hand-over.  Entry n + 8 is written after the first tile of run n + 7 was issued, that
+// is, after the tile kStages (<= 6) before it was consumed by all warps: run n is over by then.
+constexpr int kRuns = 8;
+
 template <int HD>
 struct Smem {
   uint8_t kv[Cfg<HD>::kStages][2][Cfg<HD>::kOperand];
-  float red[16][HD];
+  float red[4][4][HD];  // four rows of each warp's partial result
   uint8_t q[Cfg<HD>::kQSmem ? 64 * Cfg<HD>::kQPitch : 16];
   int scan[kMaxJobs + 1];
-  int ids[kMaxJobs];
+  int ids[kMaxPre];     // prefix jobs: group and block
+  Run run[kRuns];
   float mw[4][16], lw[4][16];
-  uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages];
+  uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages], run_full[kRuns];
   int bad[Cfg<HD>::kStages];  // 16-position blocks of the stage without a page
-  int n_pre, no_groups, abort_flag;
+  int max_cost, abort_flag;
 };
 static_assert(sizeof(Smem<128>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 128");
 static_assert(sizeof(Smem<64>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 64");
 static_assert(sizeof(Smem<256>) <= 227 * 1024, "shared memory at hd 256");
+// the ring doubles as scratch while the job list is built: row lengths, group boundaries, prefixes
+static_assert((kMaxRows + 2 * kMaxPre + 1) * sizeof(int) <= 6 * 2 * kTile * 64 * 2, "scratch");
 
-// The job list: prefix jobs in group order, then own_blocks jobs per sequence; scan[j] = tiles
-// of the jobs before j (per KV head).  All threads of the CTA.
+// The job list: scan[j] = cost of the jobs before j (per KV head), own jobs first.  All threads of the
+// CTA; everything it needs from memory is requested first, in one go.  Returns whether the groups
+// are unusable (their boundaries do not ascend inside the batch: reported, nobody shares anything).
 template <int HD>
-HM_DEV int build_jobs(const Params& P, Smem<HD>& sm) {
+HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
   const int tid = threadIdx.x, lane = tid & 31;
+  int* const len = reinterpret_cast<int*>(&sm.kv[0][0][0]);
+  int* const gs = len + kMaxRows;
+  int* const gp = gs + kMaxPre + 1;
+  const int n_own = P.B * P.own_blocks, n_jobs = P.n_jobs;
   bool bad = false;
-  for (int g = tid; g < P.n_groups; g += kThreads) bad |= bad_boundary(P, g);
+  for (int g = tid; g < P.n_groups; g += kThreads) {
+    const int a = P.gstart[g], b = P.gstart[g + 1];
+    gp[g] = group_plen(P, g);
+    gs[g] = a;
+    if (g == P.n_groups - 1) gs[g + 1] = b;
+    bad |= a < 0 || a > b || b > P.B;
+  }
+  for (int r = tid; r < P.R; r += kThreads) len[r] = row_len(P, r);
+  for (int j = n_own + tid; j < n_jobs; j += kThreads) sm.scan[j] = 0;
+  if (tid == 0) sm.max_cost = 1;
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) report_error(P.err, HM_ERR_BADINDEX);
-  if (tid < 32) {
-    int n = 0;
-    for (int g0 = 0; g0 < P.n_groups && !bad; g0 += 32) {
-      const int g = g0 + lane;
-      int jobs = 0;
-      if (g < P.n_groups && group_plen(P, g) > 0) {
-        const int rows = (P.gstart[g + 1] - P.gstart[g]) * P.S * P.G, mt = block_rows(rows);
-        jobs = (rows + mt - 1) / mt;
-      }
-      int x = jobs;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const int first = n + x - jobs;
-      for (int m = 0; m < jobs; ++m) sm.ids[first + m] = g | (m << 16);
-      if (blockIdx.x == 0 && g < P.n_groups) P.plan[kPlanGroup + g] = first;
-      n += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) {
-      sm.n_pre = n;
-      sm.no_groups = bad;
-    }
-  }
-  __syncthreads();
-  const int n_pre = sm.n_pre, n_jobs = n_pre + P.B * P.own_blocks;
-  // a block of one row: a thread per job; else eight lanes share the job's rows
+  auto put = [&](int j, const Job& J) {
+    const int c = tile_cost(J.mt), t = tiles_of(J);
+    if (t && c > 1) atomicMax(&sm.max_cost, c);
+    sm.scan[j] = t * c;
+  };
+  // eight lanes share a job's rows (one where a block is one row)
   const bool single = P.S == 1 && P.own_blocks == 1;
-  for (int j0 = 0; j0 < (single ? n_pre : n_jobs); j0 += kThreads / 8) {
-    const int j = j0 + tid / 8;
+  const int step = single ? 1 : 8, mine = tid & (step - 1);
+  for (int j0 = 0; j0 < n_own; j0 += kThreads / step) {
+    const int j = j0 + tid / step;
     Job J = {};
     int top = 0;
-    if (j < n_jobs) {
-      J = job_of(P, n_pre, sm.ids, j, bad);
-      for (int r = row_first(P, J) + (tid & 7); r <= row_last(P, J); r += 8) top = max(top, row_len(P, r));
+    if (j < n_own) {
+      const int b = P.own_blocks == 1 ? j : j / P.own_blocks;
+      const int g = bad ? -1 : group_of(gs, P.n_groups, b);
+      J = own_job(P, j - b * P.own_blocks, b, g < 0 ? 0 : gp[g]);
+      if (single)
+        top = len[b];
+      else
+        for (int r = row_first(P, J) + mine; r <= row_last(P, J); r += 8) top = max(top, len[r]);
     }
+    if (!single) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
     J.hi = min(J.hi, top);
-    if (j < n_jobs && (tid & 7) == 0) sm.scan[j] = tiles_of(J);
+    if (j < n_own && mine == 0) put(j, J);
   }
-  __syncthreads();  // the last step above may have passed n_pre: the loop below writes the same values there
-  if (single) {
-    for (int j = n_pre + tid; j < n_jobs; j += kThreads) {
-      Job J = job_of(P, n_pre, sm.ids, j, bad);
-      J.hi = min(J.hi, row_len(P, J.row0));
-      sm.scan[j] = tiles_of(J);
+  // a warp per group, eight lanes per block of its rows
+  for (int g = tid >> 5; g < P.n_groups && !bad; g += kThreads / 32) {
+    const int plen = gp[g], a = gs[g], b = gs[g + 1];
+    if (plen == 0) continue;
+    const int rows = (b - a) * P.S * P.G, mt = block_rows(rows), first = group_job(P, n_own, g, a);
+    for (int m0 = 0; m0 * mt < rows; m0 += 4) {
+      const int blk = m0 + (lane >> 3);
+      Job J = prefix_job(P, blk, a, b, plen);
+      int top = 0;
+      if (J.M > 0)
+        for (int r = row_first(P, J) + (lane & 7); r <= row_last(P, J); r += 8) top = max(top, len[r]);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      J.hi = min(J.hi, top);
+      if (J.M > 0 && (lane & 7) == 0) {
+        put(first + blk, J);
+        sm.ids[first + blk - n_own] = g | (blk << 16);
+      }
     }
   }
   __syncthreads();
@@ -301,11 +331,14 @@ HM_DEV int build_jobs(const Params& P, Smem<HD>& sm) {
     }
     if (lane == 31) sm.scan[n_jobs] = x;
   }
+  // the scratch was written by threads; TMA writes it next
+  fence_proxy_async_smem();
   __syncthreads();
-  return n_jobs;
+  return bad;
 }
 
-// The job that holds flat tile x (flat tile = scan * Hk + kh * tiles + t).
+// The job whose cost range (scan * Hk + kh * cost + tile * tile_cost) holds x: the last that starts
+// at or before it (jobs without tiles in front of it share its start).
 HM_DEV int job_at(const int* scan, int n_jobs, int64_t x, int Hk) {
   int lo = 0, hi = n_jobs - 1;
   while (lo < hi) {
@@ -315,23 +348,7 @@ HM_DEV int job_at(const int* scan, int n_jobs, int64_t x, int Hk) {
     else
       hi = mid - 1;
   }
-  return lo;  // the last with scan <= x: jobs without tiles in front of it share its offset
-}
-
-// A run of tiles [t0, t1) of one (job, KV head), part of a CTA's share.
-struct Run {
-  int j, kh, t0, t1;
-};
-HM_DEV Run run_at(const int* scan, int n_jobs, int64_t x, int64_t end, int Hk) {
-  Run r;
-  r.j = job_at(scan, n_jobs, x, Hk);
-  const int tiles = scan[r.j + 1] - scan[r.j];
-  const int64_t in = x - (int64_t)scan[r.j] * Hk;
-  r.kh = static_cast<int>(in / tiles);
-  r.t0 = static_cast<int>(in % tiles);
-  const int64_t left = end - x;
-  r.t1 = left < tiles - r.t0 ? r.t0 + static_cast<int>(left) : tiles;
-  return r;
+  return lo;
 }
 
 // ---------------------------------------------------------------- consumer
@@ -344,7 +361,7 @@ struct Consumer {
   float m[2], l[2];
   int lim[2];  // positions that this lane's two rows see
   uint32_t qf[Cfg<HD>::kQSmem ? 1 : HD / 16][4];
-  int qrow;    // first query row of this warp in shared memory
+  int qrow, part;  // first query row and position group of this warp
 
   HM_DEV Consumer(const Params& p, Smem<HD>& s) : P(p), sm(s) {
     warp = threadIdx.x >> 5;
@@ -360,13 +377,16 @@ struct Consumer {
     return reinterpret_cast<const T*>(P.q) + (int64_t)(J.row0 + v / P.G) * P.ld_q + (int64_t)(kh * P.G + v % P.G) * HD;
   }
 
-  // Query fragments, limits and cleared statistics of a run.
+  // Query fragments, limits and cleared statistics of a run.  NB: row groups of the block (1, 2, 4).
+  template <int NB>
   HM_DEV void begin(const Job& J, int kh) {
-    qrow = J.big ? warp * 16 : 0;
+    qrow = 16 * (warp & (NB - 1));
+    part = warp / NB;
+    int64_t p[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = qrow + g + 8 * e;
-      lim[e] = i < J.M ? min(row_len(P, J.row0 + (J.i0 + i) / P.G), J.hi) : J.hi;
+      p[e] = i < J.M ? row_len(P, J.row0 + (J.i0 + i) / P.G) : J.hi;
       m[e] = -INFINITY;
       l[e] = 0.f;
     }
@@ -374,8 +394,7 @@ struct Consumer {
     for (int n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     if constexpr (Cfg<HD>::kQSmem) {
       named_bar(1, kCons);  // the last run's fragments are no longer read
-      const int rows = J.big ? 64 : 16;
-      for (int c = threadIdx.x; c < rows * (HD / 8); c += kCons) {
+      for (int c = threadIdx.x; c < 16 * NB * (HD / 8); c += kCons) {
         const int i = c / (HD / 8), d = c % (HD / 8);
         const uint4 v = i < J.M ? *reinterpret_cast<const uint4*>(q_ptr(J, kh, i) + 8 * d) : make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(sm.q + i * Cfg<HD>::kQPitch + 16 * d) = v;
@@ -393,6 +412,8 @@ struct Consumer {
         qf[ks][3] = i + 8 < J.M ? *reinterpret_cast<const uint32_t*>(b + 16 * ks + 8) : 0u;
       }
     }
+    lim[0] = min(static_cast<int>(p[0]), J.hi);
+    lim[1] = min(static_cast<int>(p[1]), J.hi);
   }
 
   HM_DEV void q_frag(int ks, uint32_t (&a)[4]) const {
@@ -405,30 +426,47 @@ struct Consumer {
     }
   }
 
-  // One tile of 64 positions from p0; NB = 1: this warp's 16 positions, NB = 4: all of them.
+  // This warp's 16 * NB positions of a tile from p0 (NB = row groups of the block).
   template <int NB>
-  HM_DEV void tile(int st, int p0, const Job& J, int bad) {
-    const int b0 = NB == 1 ? warp : 0;
-    if (NB == 1 && (p0 + 16 * b0 >= J.hi || p0 + 16 * b0 + 16 <= J.lo)) return;
+  HM_DEV void tile(int st, int p0, int lo, int hi, int bad) {
+    const int b0 = NB * part;
+    if (p0 + 16 * b0 >= hi || p0 + 16 * (b0 + NB) <= lo) return;
     const uint32_t kb = smem_u32(sm.kv[st][0]), vb = smem_u32(sm.kv[st][1]);
     const int sub = 1 << P.sub_shift;                         // positions of a box: [64-dim part][position][128 bytes]
-    const uint32_t part = static_cast<uint32_t>(sub) * 128u;
+    const uint32_t half = static_cast<uint32_t>(sub) * 128u;
     // byte offset of position 16 * b of the tile in its box
     auto block_at = [&](int b) {
       const int p = 16 * b;
-      return static_cast<uint32_t>(p >> P.sub_shift) * part * (HD / 64) + static_cast<uint32_t>(p & (sub - 1)) * 128u;
+      return static_cast<uint32_t>(p >> P.sub_shift) * half * (HD / 64) + static_cast<uint32_t>(p & (sub - 1)) * 128u;
     };
     float s[2 * NB][4];
 #pragma unroll
     for (int n = 0; n < 2 * NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    {
+    if constexpr (NB == 1) {  // two sums a score: half the chain of dependent products
+      float s2[2][4] = {};
+      const int row = (mi >= 2 ? 8 : 0) + ri;
+      const uint32_t at = kb + block_at(b0) + row * 128;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t a[4], x0, x1, x2, x3;
+        q_frag(ks, a);
+        const int c = 2 * ks + (mi & 1);
+        ldsm_x4(x0, x1, x2, x3, at + (c >> 3) * half + (((c & 7) ^ ri) << 4));
+        Ty<T>::mma(ks & 1 ? s2[0] : s[0], a, x0, x1);
+        Ty<T>::mma(ks & 1 ? s2[1] : s[1], a, x2, x3);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+    } else {
       const int row = (mi >= 2 ? 8 : 0) + ri;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
         uint32_t a[4];
         q_frag(ks, a);
         const int c = 2 * ks + (mi & 1);
-        const uint32_t off = (c >> 3) * part + row * 128 + (((c & 7) ^ ri) << 4);
+        const uint32_t off = (c >> 3) * half + row * 128 + (((c & 7) ^ ri) << 4);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           uint32_t x0, x1, x2, x3;
@@ -438,7 +476,7 @@ struct Consumer {
         }
       }
     }
-    const bool edge = p0 < J.lo || p0 + kTile > J.hi || bad;  // the same for the whole CTA
+    const bool edge = p0 < lo || p0 + kTile > hi || bad;  // the same for the whole CTA
     float top[2] = {-INFINITY, -INFINITY};
     if (edge || p0 + kTile > min(lim[0], lim[1])) {
 #pragma unroll
@@ -446,7 +484,7 @@ struct Consumer {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int b = b0 + n / 2, p = p0 + 16 * b + 8 * (n & 1) + 2 * t + (e & 1);
-          const bool ok = p >= J.lo && p < lim[e >> 1] && !((bad >> b) & 1);
+          const bool ok = p >= lo && p < lim[e >> 1] && !((bad >> b) & 1);
           s[n][e] = ok ? s[n][e] * P.scale : -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
         }
@@ -497,7 +535,7 @@ struct Consumer {
       if (edge) {
         const int p = p0 + 16 * (b0 + b) + 2 * t;
         const bool no = (bad >> (b0 + b)) & 1;
-        auto in = [&](int x) { return !no && x >= J.lo && x < J.hi; };
+        auto in = [&](int x) { return !no && x >= lo && x < hi; };
         keep0 = (in(p) ? 0xffffu : 0u) | (in(p + 1) ? 0xffff0000u : 0u);
         keep1 = (in(p + 8) ? 0xffffu : 0u) | (in(p + 9) ? 0xffff0000u : 0u);
       }
@@ -507,7 +545,7 @@ struct Consumer {
       for (int nd = 0; nd < HD / 16; ++nd) {
         const int c = 2 * nd + (mi >> 1);
         uint32_t v0, v1, v2, v3;
-        ldsm_x4_t(v0, v1, v2, v3, base + (c >> 3) * part + row * 128 + (((c & 7) ^ ri) << 4));
+        ldsm_x4_t(v0, v1, v2, v3, base + (c >> 3) * half + row * 128 + (((c & 7) ^ ri) << 4));
         if (edge) {
           v0 &= keep0;
           v1 &= keep1;
@@ -521,17 +559,18 @@ struct Consumer {
   }
 
   // The run's partial result goes to rows row_at .. row_at + M - 1 of the workspace.
-  HM_DEV void finish(const Job& J, int64_t row_at) {
+  template <int NB>
+  HM_DEV void finish(int M, int64_t row_at) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
-    if (J.big) {
+    if constexpr (NB == 4) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = qrow + g + 8 * e;
-        if (i >= J.M) continue;
+        if (i >= M) continue;
         float* a = P.pa + (row_at + i) * HD + 2 * t;
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(a + 8 * n) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
@@ -540,56 +579,80 @@ struct Consumer {
           P.pl[row_at + i] = l[e];
         }
       }
-      return;
-    }
-    // the four warps' partial results, added in warp order
-    if (t == 0) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        sm.mw[warp][g + 8 * e] = m[e];
-        sm.lw[warp][g + 8 * e] = l[e];
-      }
-    }
-    named_bar(1, kCons);
-    float f[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = g + 8 * e;
-      float M = fmaxf(fmaxf(sm.mw[0][i], sm.mw[1][i]), fmaxf(sm.mw[2][i], sm.mw[3][i]));
-      const float M0 = M == -INFINITY ? 0.f : M;
-      f[e] = ex2(m[e] - M0);
-      if (warp == 0 && t == 0 && i < J.M) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) s += sm.lw[w][i] * ex2(sm.mw[w][i] - M0);
-        P.pm[row_at + i] = M;
-        P.pl[row_at + i] = s;
-      }
-    }
-    for (int w = 0; w < 4; ++w) {
-      if (warp == w) {
+    } else {
+      // the position groups of a row join with their common maximum, four rows of every warp at a time
+      if (t == 0) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (g + 8 * e >= J.M) continue;
-          float* a = &sm.red[g + 8 * e][2 * t];
+          sm.mw[warp][g + 8 * e] = m[e];
+          sm.lw[warp][g + 8 * e] = l[e];
+        }
+      }
 #pragma unroll
-          for (int n = 0; n < HD / 8; ++n) {
-            float2 x = make_float2(acc[n][2 * e] * f[e], acc[n][2 * e + 1] * f[e]);
-            float2* d = reinterpret_cast<float2*>(a + 8 * n);
-            if (w) {
-              x.x += d->x;
-              x.y += d->y;
-            }
-            *d = x;
+      for (int c = 0; c < 4; ++c) {
+        if (4 * c >= M) break;
+        if (c) named_bar(1, kCons);  // the last four rows have been read
+        if ((g >> 2) == (c & 1)) {
+          const int e = c >> 1;
+          float* a = &sm.red[warp][g & 3][2 * t];
+          if (qrow + g + 8 * e < M) {
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(a + 8 * n) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
+          }
+        }
+        named_bar(1, kCons);
+        // NB row groups x 4 rows x HD / 4 columns of 16 bytes
+        for (int x = threadIdx.x; x < NB * HD; x += kCons) {
+          const int rg = x / HD, k = x % HD / (HD / 4), i = 4 * c + k, d = 4 * (x % (HD / 4));
+          if (16 * rg + i >= M) continue;
+          float top = -INFINITY, den = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4 / NB; ++w) top = fmaxf(top, sm.mw[rg + NB * w][i]);
+          const float top0 = top == -INFINITY ? 0.f : top;
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < 4 / NB; ++w) {
+            const float f = ex2(sm.mw[rg + NB * w][i] - top0);
+            const float4 v = *reinterpret_cast<const float4*>(&sm.red[rg + NB * w][k][d]);
+            y.x += f * v.x;
+            y.y += f * v.y;
+            y.z += f * v.z;
+            y.w += f * v.w;
+            den += f * sm.lw[rg + NB * w][i];
+          }
+          const int64_t row = row_at + 16 * rg + i;
+          *reinterpret_cast<float4*>(P.pa + row * HD + d) = y;
+          if (d == 0) {
+            P.pm[row] = top;
+            P.pl[row] = den;
           }
         }
       }
-      named_bar(1, kCons);
     }
-    for (int c = threadIdx.x; c < J.M * (HD / 4); c += kCons)
-      *reinterpret_cast<float4*>(P.pa + row_at * HD + 4 * c) = *reinterpret_cast<const float4*>(&sm.red[0][0] + 4 * c);
   }
 };
+
+// A run: its query rows first (the tiles are on their way), then all of its tiles.
+template <int HD, typename T, int NB>
+HM_DEV void consume(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph) {
+  Consumer<HD, T> C(P, sm);
+  const Job J = run.J;
+  const int64_t row_at = run.prefix ? (int64_t)run.slot * P.pre_rows : P.pre_slots * P.pre_rows + (int64_t)run.slot * P.own_rows;
+  int left = run.tiles, p0 = run.tile * kTile;
+  C.template begin<NB>(J, run.kh);
+  for (; left > 0; --left, p0 += kTile) {
+    // on a timeout: carry on, the error is flagged (every warp has to reach finish's barriers)
+    mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
+    C.template tile<NB>(st, p0, J.lo, J.hi, sm.bad[st]);
+    __syncwarp();
+    if (C.lane == 0) mbar_arrive(&sm.empty[st]);
+    if (++st == Cfg<HD>::kStages) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
+  C.template finish<NB>(J.M, row_at);
+}
 
 // ---------------------------------------------------------------- kernel
 template <int HD, typename T>
@@ -603,156 +666,212 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     return;
   }
   constexpr int NST = Cfg<HD>::kStages;
+  static_assert(NST < kRuns, "run entries");
   const int tid = threadIdx.x, lane = tid & 31;
+  pdl_trigger();  // the join may be launched; it waits for this grid's end
   if (tid == 0) {
     sm.abort_flag = 0;
     for (int i = 0; i < NST; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 4);
     }
+    for (int i = 0; i < kRuns; ++i) mbar_init(&sm.run_full[i], 1);
     fence_barrier_init();
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  const int n_jobs = build_jobs(P, sm);
-  const int n_pre = sm.n_pre;
-  const bool no_groups = sm.no_groups;
-  const int64_t total = (int64_t)sm.scan[n_jobs] * P.Hk;
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t x0 = share * blockIdx.x, x1 = min(total, x0 + share);
+  const bool no_groups = build_jobs(P, sm);
+  const int n_jobs = P.n_jobs, n_own = P.B * P.own_blocks, Hk = P.Hk;
+  const int64_t total = (int64_t)sm.scan[n_jobs] * Hk;
+  // at least one tile of every kind: each CTA between a unit's first and last has one of its tiles
+  const int64_t even = (total + gridDim.x - 1) / gridDim.x, share = even > sm.max_cost ? even : sm.max_cost;
   if (blockIdx.x == 0) {  // for the join
     if (tid == 0) {
-      P.plan[0] = n_pre;
-      P.plan[1] = n_jobs;
-      P.plan[2] = static_cast<int>(share);
-      P.plan[3] = no_groups;
+      P.plan[0] = static_cast<int>(share);
+      P.plan[1] = no_groups;
     }
     for (int j = tid; j <= n_jobs; j += kThreads) P.plan[kPlanScan + j] = sm.scan[j];
   }
 
   if (tid >= kCons) {
     // ------------------------------------------------------------ producer warp
+    const int64_t x0 = share * blockIdx.x, x1 = min(total, x0 + share);
     const int sub = 1 << P.sub_shift, nsub = kTile >> P.sub_shift;
     const int batch = 32 / nsub;  // tiles whose page numbers the lanes fetch at once
-    const int none = P.n_pages * P.Hk * P.page;  // a row behind the pool: TMA fills with zeros
+    const int none = P.n_pages * Hk * P.page;  // a row behind the pool: TMA fills with zeros
     constexpr uint32_t bytes = 2 * Cfg<HD>::kOperand;
-    int it = 0;
+    int it = 0, runs = 0, st = 0, ph = 1;
     bool go = true;
-    for (int64_t x = x0; x < x1 && go;) {
-      const Run r = run_at(sm.scan, n_jobs, x, x1, P.Hk);
-      const Job J = warp_job(P, n_pre, sm.ids, r.j, no_groups);
+    auto hand_over = [&](const Run& r) {  // the entry is free: see kRuns
+      if (lane == 0) {
+        sm.run[runs % kRuns] = r;
+        mbar_arrive(&sm.run_full[runs % kRuns]);
+      }
+      ++runs;
+    };
+    int j = x0 < x1 ? job_at(sm.scan, n_jobs, x0, Hk) : n_jobs;
+    int64_t base = x0 < x1 ? (int64_t)sm.scan[j] * Hk : x1;  // where the unit (j, kh) starts
+    for (; base < x1 && go; ++j) {
+      const int cost = sm.scan[j + 1] - sm.scan[j];
+      if (cost == 0) continue;
+      int kh = 0;
+      if (base < x0) {  // the first job: the unit that holds x0
+        kh = static_cast<int>((x0 - base) / cost);
+        base += (int64_t)kh * cost;
+      }
+      Job J;
+      if (j < n_own) {
+        const int b = P.own_blocks == 1 ? j : j / P.own_blocks, g = no_groups ? -1 : group_of(P.gstart, P.n_groups, b);
+        J = own_job(P, j - b * P.own_blocks, b, g < 0 ? 0 : group_plen(P, g));
+        J.trow = P.seqs ? P.seqs[b] : b;
+      } else {
+        const int id = sm.ids[j - n_own], g = id & 0xffff;
+        J = prefix_job(P, id >> 16, P.gstart[g], P.gstart[g + 1], P.plen[g]);
+        J.trow = P.owner[g];
+      }
+      const int c = tile_cost(J.mt), tiles = cost / c;
+      // the job's tiles are known, so hi only has to be exact inside the last one
+      int top = 0;
+      for (int r = row_first(P, J) + lane; r <= row_last(P, J); r += 32) top = max(top, row_len(P, r));
+      J.hi = min(J.hi, __reduce_max_sync(0xffffffffu, top));
       const int first = J.lo / kTile;
-      for (int tb = r.t0; tb < r.t1 && go; tb += batch) {
-        const int my = tb + lane / nsub;
-        int y = none, bad = 0;
-        if (my < r.t1) {
-          const int p = (first + my) * kTile + (lane % nsub) * sub;
-          if (p + sub > J.lo && p < J.hi) {
-            const int pg = P.table[J.trow * P.table_ld + p / P.page];
-            if (pg >= 0 && pg < P.n_pages) {
-              y = (pg * P.Hk + r.kh) * P.page + p % P.page;
-            } else {
-              bad = 1;
-              report_error(P.err, HM_ERR_BADINDEX);
+      const int* const trow = P.table + J.trow * P.table_ld;
+      int have = -1, pg = 0, at = 0, bad = 0;  // the batch whose pages the lanes hold
+      for (; kh < Hk && base < x1 && go; ++kh, base += cost) {
+        const int t0 = base < x0 ? static_cast<int>((x0 - base + c - 1) / c) : 0;
+        const int t1 = x1 - base >= cost ? tiles : static_cast<int>((x1 - base + c - 1) / c);
+        if (t0 >= t1) continue;  // the share starts behind the unit's last tile's start
+        // a run is one (job, KV head) of one CTA: along the cost order either grows, so their
+        // sum numbers the runs of a kind without collisions
+        hand_over(Run{J, kh, first + t0, t1 - t0, (j < n_own ? j : j - n_own) * Hk + kh + static_cast<int>(blockIdx.x),
+                      j >= n_own});
+        for (int tb = t0; tb < t1 && go;) {
+          if (have < 0 || tb < have || tb >= have + batch) {
+            have = tb;
+            const int p = (first + tb + lane / nsub) * kTile + (lane % nsub) * sub;
+            pg = -1;
+            bad = 0;
+            at = p % P.page;
+            if (p + sub > J.lo && p < J.hi) {
+              pg = trow[p / P.page];
+              if (pg < 0 || pg >= P.n_pages) {
+                pg = -1;
+                bad = 1;
+                report_error(P.err, HM_ERR_BADINDEX);
+              }
+            }
+          }
+          const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+          const int y = pg < 0 ? none : (pg * Hk + kh) * P.page + at;
+          const int n = min(have + batch, t1) - tb;
+          for (int i = tb - have, e = i + n; i < e; ++i, ++it, ++tb) {
+            if (it >= NST) go = mbar_wait_short(&sm.empty[st], ph, P.err, &sm.abort_flag);
+            if (!__all_sync(0xffffffffu, go)) {
+              go = false;
+              break;
+            }
+            if (lane == 0) {
+              int mask = 0;  // a bit per 16 positions
+              if (bads)
+                for (int b = 0; b < kTile / 16; ++b) mask |= ((bads >> (i * nsub + ((16 * b) >> P.sub_shift))) & 1) << b;
+              sm.bad[st] = mask;
+              mbar_arrive_expect_tx(&sm.full[st], bytes);
+            }
+            __syncwarp();
+            // lane i * nsub + s holds the row of sub-box s: it issues that box of K and of V
+            if (lane / nsub == i) {
+              const int off = (lane % nsub) * sub * HD * 2;
+              tma_load_3d_plain(sm.kv[st][0] + off, &kmap, 0, y, 0, &sm.full[st]);
+              tma_load_3d_plain(sm.kv[st][1] + off, &vmap, 0, y, 0, &sm.full[st]);
+            }
+            __syncwarp();
+            if (++st == NST) {
+              st = 0;
+              ph ^= 1;
             }
           }
         }
-        const int n = min(batch, r.t1 - tb);
-        for (int i = 0; i < n; ++i, ++it) {
-          const int st = it % NST;
-          const uint32_t no = __ballot_sync(0xffffffffu, bad) >> (i * nsub);
-          int ok = 1;
-          if (lane == 0 && it >= NST) ok = mbar_wait_short(&sm.empty[st], ((it / NST) - 1) & 1, P.err, &sm.abort_flag);
-          go = __shfl_sync(0xffffffffu, ok, 0);
-          if (!go) break;
-          if (lane == 0) {
-            int mask = 0;  // a bit per 16 positions
-            for (int b = 0; b < kTile / 16; ++b) mask |= ((no >> ((16 * b) >> P.sub_shift)) & 1) << b;
-            sm.bad[st] = mask;
-            mbar_arrive_expect_tx(&sm.full[st], bytes);
-          }
-          __syncwarp();
-          // lane i * nsub + s holds the row of sub-box s: it issues that box of K and of V
-          if (lane / nsub == i) {
-            const int s = lane % nsub, off = s * sub * HD * 2;
-            tma_load_3d_plain(sm.kv[st][0] + off, &kmap, 0, y, 0, &sm.full[st]);
-            tma_load_3d_plain(sm.kv[st][1] + off, &vmap, 0, y, 0, &sm.full[st]);
-          }
-          __syncwarp();
-        }
       }
-      x += r.t1 - r.t0;
     }
+    hand_over(Run{});  // no tiles: the end
   } else {
     // ------------------------------------------------------------ consumers
-    Consumer<HD, T> C(P, sm);
-    int it = 0;
-    for (int64_t x = x0; x < x1;) {
-      const Run r = run_at(sm.scan, n_jobs, x, x1, P.Hk);
-      const Job J = warp_job(P, n_pre, sm.ids, r.j, no_groups);
-      C.begin(J, r.kh);
-      const int first = J.lo / kTile;
-      for (int tt = r.t0; tt < r.t1; ++tt, ++it) {
-        const int st = it % NST;
-        mbar_wait_short(&sm.full[st], (it / NST) & 1, P.err, &sm.abort_flag);  // on timeout: carry on, error flagged
-        const int bad = sm.bad[st], p0 = (first + tt) * kTile;
-        if (J.big)
-          C.template tile<4>(st, p0, J, bad);
-        else
-          C.template tile<1>(st, p0, J, bad);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[st]);
-      }
-      // a run is one (job, KV head) of one CTA: along the flat order either grows, so their sum
-      // numbers the runs of a kind without collisions
-      const int64_t slot = (int64_t)(r.j < n_pre ? r.j : r.j - n_pre) * P.Hk + r.kh + blockIdx.x;
-      C.finish(J, r.j < n_pre ? slot * P.pre_rows : P.pre_slots * P.pre_rows + slot * P.own_rows);
-      x += r.t1 - r.t0;
+    int st = 0, ph = 0;
+    for (int n = 0;; ++n) {
+      const bool ok = mbar_wait_short(&sm.run_full[n % kRuns], (n / kRuns) & 1, P.err, &sm.abort_flag);
+      // after a timeout (flagged) all four warps stop together: none waits for another at a barrier
+      if (named_bar_or(1, kCons, !ok)) break;
+      const Run& run = sm.run[n % kRuns];
+      if (run.tiles == 0) break;
+      if (run.J.mt == 16)
+        consume<HD, T, 1>(P, sm, run, st, ph);
+      else if (run.J.mt == 32)
+        consume<HD, T, 2>(P, sm, run, st, ph);
+      else
+        consume<HD, T, 4>(P, sm, run, st, ph);
     }
   }
-  pdl_trigger();
 }
 
-// Joins the partial results of a (row, head), one warp each: the prefix's in order, then the
-// sequence's own.  Nothing to join (a padding row): zeros.
+// Joins the partial results of a (row, head), one warp each: the sequence's own in order, then the
+// prefix's.  Nothing to join (a padding row): zeros.
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params P) {
-  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (id >= (int64_t)P.R * P.Hq) return;
-  const int r = static_cast<int>(id / P.Hq), h = static_cast<int>(id % P.Hq), kh = h / P.G;
-  const int n_pre = P.plan[0], b = r / P.S;
-  const int64_t share = P.plan[2];
-  const int* scan = P.plan + kPlanScan;
-  int64_t at[2] = {0, 0}, step[2] = {P.pre_rows, P.own_rows};  // workspace row of the first split, distance of the next
-  int cnt[2] = {0, 0};
-  auto splits = [&](int j, int unit, int row, int kind) {
-    const int tiles = scan[j + 1] - scan[j];
-    if (tiles == 0) return;
-    const int64_t x = (int64_t)scan[j] * P.Hk + (int64_t)kh * tiles;
-    const int64_t c0 = x / share, c1 = (x + tiles - 1) / share;
-    cnt[kind] = static_cast<int>(c1 - c0) + 1;
-    at[kind] = (kind ? P.pre_slots * P.pre_rows : 0) + ((int64_t)unit * P.Hk + kh + c0) * step[kind] + row;
-  };
-  const int g = P.plan[3] ? -1 : group_of(P, b);
+  const bool live = id < (int64_t)P.R * P.Hq;
+  const int r = live ? static_cast<int>(id / P.Hq) : 0, h = static_cast<int>(id % P.Hq), kh = h / P.G, b = r / P.S;
+  // the call's inputs do not change while it runs: read them while the first kernel still works
+  int g = group_of(P.gstart, P.n_groups, b), i = 0, mt = 16, j = 0;
   if (g >= 0 && group_plen(P, g) > 0) {
-    const int a = P.gstart[g], mt = block_rows((P.gstart[g + 1] - a) * P.S * P.G);
-    const int i = (r - a * P.S) * P.G + h % P.G, j = P.plan[kPlanGroup + g] + i / mt;
-    splits(j, j, i % mt, 0);
+    const int a = P.gstart[g];
+    mt = block_rows((P.gstart[g + 1] - a) * P.S * P.G);
+    i = (r - a * P.S) * P.G + h % P.G;
+    j = group_job(P, P.B * P.own_blocks, g, a) + i / mt;
+  } else {
+    g = -1;
   }
-  {
-    const int mt = block_rows(P.S * P.G), i = (r % P.S) * P.G + h % P.G;
-    const int u = b * P.own_blocks + i / mt;
-    splits(n_pre + u, u, i % mt, 1);
-  }
+  const int omt = block_rows(P.S * P.G), oi = (r % P.S) * P.G + h % P.G, u = b * P.own_blocks + oi / omt;
+  pdl_wait();
+  if (!live) return;
+  const int* scan = P.plan + kPlanScan;
+  const int64_t share = P.plan[0];
+  if (P.plan[1]) g = -1;
+  int64_t at[2] = {0, 0};  // workspace row of the first split; the next one is a slot further
+  int cnt[2] = {0, 0};
+  auto splits = [&](int j, int unit, int row, int c, int kind) {
+    const int s0 = scan[j], cost = scan[j + 1] - s0;
+    if (cost == 0) return;
+    const int64_t x = (int64_t)s0 * P.Hk + (int64_t)kh * cost;
+    const int64_t c0 = x / share, c1 = (x + cost - c) / share;
+    cnt[kind] = static_cast<int>(c1 - c0) + 1;
+    at[kind] = ((int64_t)unit * P.Hk + kh + c0) * (kind ? P.pre_rows : P.own_rows) + row +
+               (kind ? 0 : P.pre_slots * P.pre_rows);
+  };
+  splits(u, u, oi % omt, tile_cost(omt), 0);
+  if (g >= 0) splits(j, j - P.B * P.own_blocks, i % mt, tile_cost(mt), 1);
   const int n = cnt[0] + cnt[1];
-  auto row_of = [&](int s) { return s < cnt[0] ? at[0] + s * step[0] : at[1] + (s - cnt[0]) * step[1]; };
+  auto row_of = [&](int s) {
+    return s < cnt[0] ? at[0] + (int64_t)s * P.own_rows : at[1] + (int64_t)(s - cnt[0]) * P.pre_rows;
+  };
+  constexpr int V = HD / 32, E = 4;  // columns of a lane; splits whose columns are requested at once
+  auto cols = [&](int s, float (&a)[V]) {
+    const float* p = P.pa + row_of(s) * HD + V * lane;
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 f = *reinterpret_cast<const float2*>(p + e);
+      a[e] = f.x;
+      a[e + 1] = f.y;
+    }
+  };
+  float early[E][V];  // before the maxima are known: one latency less
+#pragma unroll
+  for (int s = 0; s < E; ++s)
+    if (s < n) cols(s, early[s]);
   float M = -INFINITY;
   for (int s = lane; s < n; s += 32) M = fmaxf(M, P.pm[row_of(s)]);
   M = warp_max(M);
   const float M0 = M == -INFINITY ? 0.f : M;
-  constexpr int V = HD / 32;  // columns of a lane
   float num[V] = {};
   float den = 0.f;
   for (int s0 = 0; s0 < n; s0 += 32) {
@@ -764,21 +883,34 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
     }
     den += warp_sum(ls);
     const int e = min(32, n - s0);
-#pragma unroll 4
-    for (int s = 0; s < e; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float* a = P.pa + row_of(s0 + s) * HD + V * lane;
+    int s = 0;
+    if (s0 == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) num[i] += ws * a[i];
+      for (int k = 0; k < E; ++k) {
+        const float ws = __shfl_sync(0xffffffffu, w, k);
+        if (k < n) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) num[v] += ws * early[k][v];
+        }
+      }
+      s = E;
+    }
+#pragma unroll 4
+    for (; s < e; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      float a[V];
+      cols(s0 + s, a);
+#pragma unroll
+      for (int v = 0; v < V; ++v) num[v] += ws * a[v];
     }
   }
-  const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);  // NaN stays NaN
+  const float inv = 1.f / den;  // NaN stays NaN
   uint32_t out[V / 2];
 #pragma unroll
-  for (int i = 0; i < V; i += 2) out[i / 2] = Ty<T>::pack(den == 0.f ? 0.f : num[i] * inv, den == 0.f ? 0.f : num[i + 1] * inv);
+  for (int v = 0; v < V; v += 2) out[v / 2] = den == 0.f ? 0u : Ty<T>::pack(num[v] * inv, num[v + 1] * inv);
   uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(P.o) + r * P.ld_o + (int64_t)h * HD + V * lane);
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) o[i] = out[i];
+  for (int v = 0; v < V / 2; ++v) o[v] = out[v];
 }
 
 // ---------------------------------------------------------------- host side
@@ -792,15 +924,15 @@ bool shape_of(int R, int S, int Hq, int Hk, int n_groups, int ctas, Shape* s) {
   if (R < 1 || S < 1 || R % S || Hk < 1 || Hq < Hk || Hq % Hk || n_groups < 0) return false;
   s->B = R / S;
   s->G = Hq / Hk;
-  if (s->G > 64 || R > (1 << 20)) return false;
+  if (s->G > 64 || R > kMaxRows) return false;
   const int64_t own = (int64_t)S * s->G, all = (int64_t)R * s->G;
-  const int own_mt = own <= 16 ? 16 : 64;
+  const int own_mt = block_rows(static_cast<int>(own > 64 ? 64 : own));
   s->own_blocks = static_cast<int>((own + own_mt - 1) / own_mt);
   s->own_rows = static_cast<int>(own < own_mt ? own : own_mt);
-  s->pre_rows = all <= 16 ? static_cast<int>(all) : 64;
-  // groups of up to 16 rows are one job, larger ones one per started 64 rows
-  s->pre_jobs = n_groups == 0 ? 0 : (all + 63) / 64 + n_groups;
-  if (s->pre_jobs + (int64_t)s->B * s->own_blocks > kMaxJobs || n_groups > kMaxJobs) return false;
+  s->pre_rows = static_cast<int>(all < 64 ? all : 64);
+  // groups of up to 64 rows are one job, larger ones one per started 64 rows
+  s->pre_jobs = n_groups == 0 ? 0 : all / 64 + n_groups;
+  if (s->pre_jobs + (int64_t)s->B * s->own_blocks > kMaxJobs || s->pre_jobs > kMaxPre) return false;
   s->pre_slots = s->pre_jobs ? s->pre_jobs * Hk + ctas : 0;
   s->rows = s->pre_slots * s->pre_rows + ((int64_t)s->B * s->own_blocks * Hk + ctas) * s->own_rows;
   return true;
@@ -821,7 +953,7 @@ cudaError_t device_sms(int* dev, int* sms) {
 
 int ctas_per_sm(int hd) { return hd <= 128 ? 2 : 1; }
 
-size_t plan_bytes(int n_groups) { return ((kPlanGroup + n_groups) * sizeof(int) + 255) / 256 * 256; }
+constexpr size_t kPlanBytes = (kPlanInts * sizeof(int) + 255) / 256 * 256;
 
 // [rows of the pool, hd] as {64 dims, rows, hd / 64}, a box of `sub` rows and all dims
 bool pool_map(const void* p, int64_t rows, int hd, int sub, bool bf16, CUtensorMap* out) {
@@ -866,7 +998,7 @@ extern "C" size_t hm_prefix_attn_workspace_bytes(int R, int S, int Hq, int Hk, i
   Shape s;
   if ((hd != 64 && hd != 128 && hd != 256) || sms < 1 || !shape_of(R, S, Hq, Hk, n_groups, sms * ctas_per_sm(hd), &s))
     return 0;
-  return plan_bytes(n_groups) + (size_t)s.rows * (hd + 2) * sizeof(float) + 16;
+  return kPlanBytes + (size_t)s.rows * (hd + 2) * sizeof(float) + 16;
 }
 
 extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) {
@@ -880,8 +1012,8 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
   // pool rows and positions are 32-bit TMA coordinates / lengths
   if ((int64_t)d->n_pages * d->Hk * pg > 0x7fffff00 || (int64_t)d->max_pages * pg > 0x7fffff00) return HM_EARG;
   if (d->ld_q % 8 || d->ld_o % 8 || d->ld_q < (int64_t)d->Hq * d->hd || d->ld_o < (int64_t)d->Hq * d->hd) return HM_EARG;
-  // tile offsets are 32-bit
-  if (((int64_t)d->max_pages * pg / kTile + 1) * kMaxJobs > 0x7fffffff) return HM_EARG;
+  // costs are 32-bit
+  if (((int64_t)d->max_pages * pg / kTile + 1) * tile_cost(64) * kMaxJobs > 0x7fffffff) return HM_EARG;
   // before anything asks for the device: the sizes do not depend on the number of SMs
   Shape s;
   if (!shape_of(d->R, d->S, d->Hq, d->Hk, d->n_groups, 1, &s)) return HM_EARG;
@@ -922,12 +1054,13 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
   p.n_groups = d->n_groups;
   p.sub_shift = sub == 16 ? 4 : (sub == 32 ? 5 : 6);
   p.scale = d->scale * 1.4426950408889634f;
+  p.n_jobs = static_cast<int>(s.B * (int64_t)s.own_blocks + s.pre_jobs);
   p.own_blocks = s.own_blocks;
   p.own_rows = s.own_rows;
   p.pre_rows = s.pre_rows;
   p.pre_slots = s.pre_slots;
   p.plan = reinterpret_cast<int*>(d->ws);
-  p.pa = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(d->ws) + plan_bytes(d->n_groups));
+  p.pa = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(d->ws) + kPlanBytes);
   p.pm = p.pa + s.rows * d->hd;
   p.pl = p.pm + s.rows;
   p.err = d->err;

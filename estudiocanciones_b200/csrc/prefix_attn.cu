@@ -998,7 +998,7 @@ extern "C" size_t hm_prefix_attn_workspace_bytes(int R, int S, int Hq, int Hk, i
   Shape s;
   if ((hd != 64 && hd != 128 && hd != 256) || sms < 1 || !shape_of(R, S, Hq, Hk, n_groups, sms * ctas_per_sm(hd), &s))
     return 0;
-  return kPlanBytes + (size_t)s.rows * (hd + 2) * sizeof(float) + 16;
+  return kPlanBytes + (size_t)s.rows * (hd + 2) * sizeof(float);
 }
 
 extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) {

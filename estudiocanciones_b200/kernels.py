@@ -257,6 +257,8 @@ def prefill_attn(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, P: int, o:
 # are built only when a check fails, the stream is read as a raw handle, and the device is
 # switched only when the tensors lie on another one than the current.
 _DT = {torch.float16: _lib.HM_DT_F16, torch.bfloat16: _lib.HM_DT_BF16}
+_I32, _I64, _F16 = torch.int32, torch.int64, torch.float16
+_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _ERR_PTRS: dict[int, int] = {}
 
 
@@ -277,14 +279,19 @@ def _err_ptr(idx: int) -> int:
     return p
 
 
+_FNS: dict = {}
+
+
 def _launch(idx: int, what: str, *args) -> None:
     """The entry point ``what`` with ``args`` on the current stream of device ``idx``."""
-    fn = getattr(_lib.lib(), what)
-    if torch._C._cuda_getDevice() == idx:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    fn = _FNS.get(what)
+    if fn is None:
+        fn = _FNS[what] = getattr(_lib.lib(), what)
+    if _get_device() == idx:
+        rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+            rc = fn(*args, _raw_stream(idx))
     if rc:
         check(rc, what)
 
@@ -312,26 +319,29 @@ def _ids(what: str, ids, like) -> torch.Tensor:
     return ids
 
 
-def _is_table(t) -> bool:
-    return (t.dtype == torch.int32 and t.dim() == 2 and t.numel() > 0 and t.stride(1) == 1 and
-            t.stride(0) >= t.shape[1])
+def _table(what: str, t):
+    """(sequences, pages of a row, row pitch) of a page table."""
+    shape = t.shape
+    if t.dtype == _I32 and len(shape) == 2:
+        n, mp = shape
+        ld, one = t.stride()
+        if one == 1 and ld >= mp and n > 0 and mp > 0:
+            return n, mp, ld
+    raise HMError(f"{what}: table is int32 [sequences, pages], rows contiguous")
 
 
 def _page_state(what: str, table, lens, refs, page: int):
     """(device index, hm_page_state).  ``lens`` None: a call that does not read it."""
     idx = _device_of(what, table, lens, refs)
-    if not _is_table(table):
-        raise HMError(f"{what}: table is int32 [sequences, pages], rows contiguous")
-    n, mp = table.shape
-    if lens is not None and (lens.dtype != torch.int64 or lens.dim() != 1 or lens.numel() != n or
-                             not lens.is_contiguous()):
+    n, mp, ld = _table(what, table)
+    if lens is not None and (lens.dtype != _I64 or lens.shape != (n,) or not lens.is_contiguous()):
         raise HMError(f"{what}: lens is int64 [sequences]")
     n_pages = refs.numel()
-    if refs.dtype != torch.int32 or refs.dim() != 1 or n_pages < 1 or not refs.is_contiguous():
+    if refs.dtype != _I32 or refs.dim() != 1 or n_pages < 1 or not refs.is_contiguous():
         raise HMError(f"{what}: refs is int32 [pages of the pool]")
     if not 1 <= page <= 1024:
         raise HMError(f"{what}: a page holds 1 to 1024 positions")
-    return idx, _lib.PACK_PAGE_STATE.pack(table.data_ptr(), table.stride(0), 0 if lens is None else lens.data_ptr(),
+    return idx, _lib.PACK_PAGE_STATE.pack(table.data_ptr(), ld, 0 if lens is None else lens.data_ptr(),
                                           refs.data_ptr(), _err_ptr(idx), n, mp, n_pages, page)
 
 
@@ -421,21 +431,21 @@ def pages_compact(k, v, table, refs) -> torch.Tensor:
 
 
 def _layer_pages(what: str, k, v, table, seqs, R: int, S: int):
-    """One layer's pool and the rows of its table that R query rows use; returns the pool's shape."""
+    """One layer's pool and the rows of its table that R query rows use; returns the pool's shape and
+    the table's."""
     shape, dt = k.shape, k.dtype
     if (dt not in _DT or len(shape) != 4 or v.shape != shape or v.dtype != dt or not k.is_contiguous() or
             not v.is_contiguous() or k.numel() == 0):
         raise HMError(f"{what}: k and v are contiguous fp16 or bf16 [pages, Hk, page, hd]")
-    if not _is_table(table):
-        raise HMError(f"{what}: table is int32 [sequences, pages], rows contiguous")
+    tab = _table(what, table)
     if S < 1 or R < 1 or R % S:
         raise HMError(f"{what}: S >= 1 rows of every sequence")
     if seqs is None:
-        if R // S > table.shape[0]:
+        if R // S > tab[0]:
             raise HMError(f"{what}: the table has a row for every sequence")
-    elif seqs.dtype != torch.int32 or seqs.shape != (R // S,) or not seqs.is_contiguous():
+    elif seqs.dtype != _I32 or seqs.shape != (R // S,) or not seqs.is_contiguous():
         raise HMError(f"{what}: seqs is int32 [sequences]")
-    return shape
+    return shape, tab
 
 
 def _is_rows(t, R: int, W: int) -> bool:
@@ -449,7 +459,7 @@ def rope_pages(qkv, rope, pos, q_out, k, v, table, S: int, Hq: int, Hk: int, seq
     A padding row has ``pos[r] < 0``: its ``q_out`` is zero and nothing is written."""
     idx = _device_of("rope_pages", qkv, rope, pos, q_out, k, v, table, seqs)
     R = qkv.shape[0]
-    n_pages, hk, page, hd = _layer_pages("rope_pages", k, v, table, seqs, R, S)
+    (n_pages, hk, page, hd), (n_table, max_pages, ld) = _layer_pages("rope_pages", k, v, table, seqs, R, S)
     if hk != Hk or hd % 8:
         raise HMError("rope_pages: Hk heads of a multiple of 8 dims")
     if qkv.dtype != k.dtype or q_out.dtype != k.dtype or not _is_rows(qkv, R, (Hq + 2 * Hk) * hd):
@@ -462,8 +472,8 @@ def rope_pages(qkv, rope, pos, q_out, k, v, table, S: int, Hq: int, Hk: int, seq
         raise HMError("rope_pages: pos is int64 [R]")
     _launch(idx, "hm_rope_pages", qkv.data_ptr(), qkv.stride(0) if R > 1 else qkv.shape[1], rope.data_ptr(),
             rope.shape[0], pos.data_ptr(), q_out.data_ptr(), q_out.stride(0) if R > 1 else q_out.shape[1],
-            k.data_ptr(), v.data_ptr(), _DT[k.dtype], table.data_ptr(), table.stride(0),
-            None if seqs is None else seqs.data_ptr(), table.shape[0], table.shape[1], n_pages, page, R, S, Hq, Hk, hd,
+            k.data_ptr(), v.data_ptr(), _DT[k.dtype], table.data_ptr(), ld,
+            None if seqs is None else seqs.data_ptr(), n_table, max_pages, n_pages, page, R, S, Hq, Hk, hd,
             _err_ptr(idx))
 
 
@@ -493,23 +503,23 @@ def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int 
     if q.dim() != 2:
         raise HMError("prefix_attn: q [R, Hq * hd]")
     R, W = q.shape
-    n_pages, Hk, page, hd = _layer_pages("prefix_attn", k, v, table, seqs, R, S)
+    (n_pages, Hk, page, hd), (n_table, max_pages, ld) = _layer_pages("prefix_attn", k, v, table, seqs, R, S)
     Hq, dt = W // hd, q.dtype
-    if dt != k.dtype or W != Hq * hd or Hq < Hk or Hq % Hk or q.stride(1) != 1:
+    ld_q, one = q.stride()
+    if dt != k.dtype or W != Hq * hd or Hq < Hk or Hq % Hk or one != 1:
         raise HMError("prefix_attn: q [R, Hq * hd] of the cache's type, Hq a multiple of Hk")
     if o is None:
-        o = torch.empty((R, W), dtype=dt, device=q.device)
+        o = q.new_empty((R, W))
     elif o.dtype != dt or not _is_rows(o, R, W):
         raise HMError("prefix_attn: o is like q")
-    if pos.dtype != torch.int64 or pos.dim() != 1 or pos.numel() != R or not pos.is_contiguous():
+    if pos.dtype != _I64 or pos.shape != (R,) or not pos.is_contiguous():
         raise HMError("prefix_attn: pos is int64 [R]")
     groups = gs = ow = pl = 0
     if gstart is not None:
         groups = gstart.numel() - 1
         if owner is None or plen is None:
             raise HMError("prefix_attn: gstart comes with owner and plen")
-        i32 = torch.int32
-        if (groups < 0 or gstart.dtype != i32 or owner.dtype != i32 or plen.dtype != i32 or gstart.dim() != 1 or
+        if (groups < 0 or gstart.dtype != _I32 or owner.dtype != _I32 or plen.dtype != _I32 or gstart.dim() != 1 or
                 owner.shape != (groups,) or plen.shape != (groups,) or not gstart.is_contiguous() or
                 not owner.is_contiguous() or not plen.is_contiguous()):
             raise HMError("prefix_attn: gstart [groups + 1], owner and plen [groups] are int32 vectors")
@@ -520,10 +530,9 @@ def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int 
     nbytes = _size("hm_prefix_attn_workspace_bytes", R, S, Hq, Hk, hd, groups, _sms(idx))
     if nbytes == 0:
         raise HMError("prefix_attn: hd 64, 128 or 256, up to 64 query heads per KV head and 1024 row blocks")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    n_table, max_pages = table.shape
-    d = _lib.PACK_PREFIX_ATTN.pack(q.data_ptr(), q.stride(0) if R > 1 else W, o.data_ptr(), o.stride(0) if R > 1 else W,
-                                   k.data_ptr(), v.data_ptr(), pos.data_ptr(), table.data_ptr(), table.stride(0),
+    ws = q.new_empty(nbytes // 2)   # (16-bit elements)
+    d = _lib.PACK_PREFIX_ATTN.pack(q.data_ptr(), ld_q if R > 1 else W, o.data_ptr(), o.stride(0) if R > 1 else W,
+                                   k.data_ptr(), v.data_ptr(), pos.data_ptr(), table.data_ptr(), ld,
                                    0 if seqs is None else seqs.data_ptr(), gs, ow, pl, ws.data_ptr(), nbytes,
                                    _err_ptr(idx), _DT[dt], R, S, Hq, Hk, hd, n_table, max_pages, n_pages, page, groups,
                                    1.0 / math.sqrt(hd) if scale is None else scale)
@@ -539,7 +548,8 @@ def _rows16(what: str, x) -> torch.Tensor:
     K = x.shape[1]
     if K < 16 or K % 16 or K > 131072:
         raise HMError(f"{what}: K a multiple of 16, at most 131072")
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < K)):
+    ld, one = x.stride()
+    if one != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (ld % 8 or ld < K)):
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -551,10 +561,12 @@ def _pitch(t) -> int:
 
 def _a8_out(what: str, dtype, w, s, res, out, silu: bool, M: int, K: int, device):
     """Checks of the weights and outputs; returns (N, out)."""
-    if w.dtype != torch.int8 or w.dim() != 2 or w.shape[1] != K or w.shape[0] < 1 or not w.is_contiguous():
+    if w.dtype != torch.int8 or w.dim() != 2 or not w.is_contiguous():
         raise HMError(f"{what}: w is contiguous int8 [N, K]")
-    N = w.shape[0]
-    if s.dtype != torch.float16 or s.dim() != 1 or s.numel() != N or not s.is_contiguous():
+    N, wk = w.shape
+    if wk != K or N < 1:
+        raise HMError(f"{what}: w [N, K] has a row per output column and the activations' K")
+    if s.dtype != _F16 or s.shape != (N,) or not s.is_contiguous():
         raise HMError(f"{what}: s is fp16 [N]")
     if silu and (res is not None or N % 2):
         raise HMError(f"{what}: silu takes w = [w1; w3] and no residual")
@@ -562,7 +574,7 @@ def _a8_out(what: str, dtype, w, s, res, out, silu: bool, M: int, K: int, device
     if res is not None and (res.dtype != dtype or not _is_rows(res, M, nout)):
         raise HMError(f"{what}: res [M, N] of the activations' type")
     if out is None:
-        out = torch.empty(M, nout, dtype=dtype, device=device)
+        out = s.new_empty((M, nout)) if dtype == _F16 else torch.empty(M, nout, dtype=dtype, device=device)
     elif out.dtype != dtype or not _is_rows(out, M, nout):
         raise HMError(f"{what}: out [M, N] of the activations' type")
     return N, out
@@ -614,7 +626,7 @@ def int8_mm_a8(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, res: torch.Ten
     M, K = x.shape
     N, out = _a8_out("int8_mm_a8", x.dtype, w, s, res, out, silu, M, K, x.device)
     nbytes = _size("hm_int8_mm_a8_workspace_bytes", M, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    ws = w.new_empty(nbytes)
     _launch(idx, "hm_int8_mm_a8", x.data_ptr(), _pitch(x), _DT[x.dtype], w.data_ptr(), s.data_ptr(),
             None if res is None else res.data_ptr(), 0 if res is None else _pitch(res), out.data_ptr(), _pitch(out), M,
             N, K, _lib.HM_EPI_SILU if silu else _lib.HM_EPI_STORE, ws.data_ptr(), nbytes, _err_ptr(idx))

@@ -9,31 +9,38 @@
 // which join exactly: with M = max m_i,  o = sum_i a_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
 //
 // What bounds it: K and V are read once per group and once per sequence, 4 * Hk * hd bytes a
-// position, against 4 * Hq * hd operations a (row, position).  Up to ~100 query rows per KV head
-// that is less than the tensor cores do while the bytes arrive, so the kernel is built to keep
-// the memory busy:
+// position, against 4 * Hq * hd operations a (row, position).  The kernel is built to keep the
+// memory busy and the tensor cores off the critical path:
 //  * The work is a list of jobs (one sequence's own positions or a group's prefix, cut into blocks
 //    of query rows) x KV heads x tiles of 64 positions.  Lengths live on the device, so every CTA
 //    builds the list itself (one pass over pos, a scan in shared memory) and takes an equal share
-//    of the cost: a long prefix next to short sequences leaves no SM idle, whatever the lengths.
+//    of the tiles: a long prefix next to short sequences leaves no SM idle, whatever the lengths.
 //  * One producer warp fetches page numbers 32 at a time and issues one TMA box per page and
 //    operand (128-byte swizzle) into a ring of 96 KB per CTA, two CTAs per SM, across job
 //    boundaries, so the ring never drains.  It also works out what each run of tiles belongs to
-//    and hands that over with the run's first tile.
-//  * Four consumer warps share a block of query rows (the G heads of a KV head x rows) as
-//    row groups x position groups: 16 rows: 1 x 4 (K and V leave shared memory once), 32 rows:
-//    2 x 2, 64 rows: 4 x 1.  Position groups meet in shared memory at the end of a run.
+//    and hands that over before the tiles arrive.
+//  * Blocks of up to 16 query rows (the G heads of a KV head x rows; every sequence's own positions
+//    in a decode step): mma.sync, each of the four consumer warps takes 16 of the tile's
+//    positions, so K and V leave shared memory once; the four partial results meet there.
+//  * Blocks of up to 128 rows (a prefix and the rows that share it): tcgen05.  Q and the
+//    probabilities are the TMEM operands A of S = Q K^T and O += P V, K and V are read where TMA put
+//    them; one thread per row does the softmax.  P replaces S in TMEM, so S, Q and O of a CTA take
+//    256 columns (hd 128) and two CTAs share an SM: one's softmax runs beside the other's products.
+//    O is rescaled only when a row's maximum has grown by more than 2^8 (its reference stays a
+//    little behind: P <= 256, the result does not depend on it), which is rare after a few tiles.
+//    A 64-row tile took 4500 cycles with mma.sync and one warp per 16 rows.
 //  * A second small kernel joins the partial results of a row in a fixed order (results do not
 //    depend on scheduling) and writes o; its launch overlaps the first kernel's tail.
 // Scores, m, l and a are fp32; the probabilities are rounded to the cache's type for the product
-// with V, as the flat decode attention does (they are at most 1; l keeps the unrounded sum).
-// V rows outside a job's range are zeroed in registers, so whatever stands there (NaN included)
-// has no effect.
+// with V, as the flat decode attention does (l keeps the unrounded sum).  V rows outside a job's
+// range are zeroed (in registers, in shared memory for tcgen05), so whatever stands there (NaN
+// included) has no effect.
 #include <cuda_bf16.h>
 
 #include <atomic>
 
 #include "hm_common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -41,8 +48,9 @@ constexpr int kTile = 64;       // positions per tile
 constexpr int kMaxJobs = 1024;  // jobs of a call (the list lives in shared memory)
 constexpr int kMaxPre = 896;    // prefix jobs, and groups, of a call
 constexpr int kMaxRows = 16384; // query rows of a call
-constexpr int kThreads = 160;   // 4 consumer warps + the producer
+constexpr int kThreads = 192;   // 4 consumer warps, the producer, the tcgen05 issuer
 constexpr int kCons = 128;
+constexpr int kBig = 128;       // rows of a tcgen05 block
 
 struct Params {
   const void* q;
@@ -63,6 +71,7 @@ struct Params {
   int own_blocks;     // row blocks of one sequence's own job
   int own_rows;       // row capacity of an own partial
   int pre_rows;       // row capacity of a prefix partial
+  int big;            // some block may have more than 16 rows
   int64_t pre_slots;  // prefix partials come first
   int* plan;          // what the join needs of the job list
   float* pm;          // [rows] maxima, [rows] sums, [rows][hd] accumulators
@@ -71,7 +80,7 @@ struct Params {
   int* err;
 };
 
-// plan: 0 a CTA's share of the cost, 1 groups unusable; then the cost before every job
+// plan: 0 a CTA's share of the tiles, 1 groups unusable; then the tiles before every job (per KV head)
 constexpr int kPlanScan = 2, kPlanInts = 2 + kMaxJobs + 1;
 #define HM_HD __host__ __device__ __forceinline__
 
@@ -80,6 +89,7 @@ template <typename T>
 struct Ty;
 template <>
 struct Ty<__half> {
+  static constexpr uint32_t kFormat = 0;  // of tcgen05 operands A and B
   static HM_DEV uint32_t pack(float a, float b) { return pack_h2(a, b); }
   static HM_DEV void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -87,6 +97,7 @@ struct Ty<__half> {
 };
 template <>
 struct Ty<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
   static HM_DEV uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -121,11 +132,7 @@ HM_DEV float ex2(float x) {
 
 // ---------------------------------------------------------------- lengths and groups
 // Block size of a job with `rows` query rows per KV head.
-HM_HD int block_rows(int rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
-// What a tile costs a CTA: up to 32 rows its bytes (about 2800 cycles at an even share of HBM, the
-// arithmetic takes 1600 or 2300), with 64 rows the arithmetic (4200).
-HM_HD int tile_cost(int mt) { return mt <= 32 ? 2 : 3; }
-
+HM_HD int block_rows(int rows) { return rows <= 16 ? 16 : kBig; }
 // Positions that row r attends to: 0 for a padding row and for one whose position or table row
 // is out of range (reported).
 HM_DEV int row_len(const Params& P, int r) {
@@ -170,8 +177,8 @@ struct Job {
 };
 
 // The first prefix job of a group whose sequences start at a: a group of n rows has at most
-// n / 64 + 1 jobs, so these numbers leave room for all of them without a scan.
-HM_DEV int group_job(const Params& P, int n_own, int g, int a) { return n_own + ((a * P.S * P.G) >> 6) + g; }
+// n / 128 + 1 jobs, so these numbers leave room for all of them without a scan.
+HM_DEV int group_job(const Params& P, int n_own, int g, int a) { return n_own + a * P.S * P.G / kBig + g; }
 
 // Block blk of group g's prefix (sequences a .. b - 1), and of sequence b's own positions behind a
 // prefix of lo.  hi is not yet cut to what the rows see.
@@ -206,10 +213,13 @@ HM_DEV int tiles_of(const Job& J) { return J.hi > J.lo ? (J.hi - 1) / kTile - J.
 template <int HD>
 struct Cfg {
   static constexpr int kOperand = kTile * HD * 2;  // bytes of a K (or V) tile
-  static constexpr int kStages = HD == 64 ? 6 : (HD == 128 ? 3 : 2);
+  static constexpr int kStages = HD == 64 ? 6 : 3;
   static constexpr int kCtas = HD <= 128 ? 2 : 1;  // per SM
   static constexpr bool kQSmem = HD > 128;         // query fragments: registers, or shared memory
   static constexpr int kQPitch = HD * 2 + 16;
+  // TMEM columns of a tcgen05 block: S (then P) 64, Q hd / 2, O hd
+  static constexpr uint32_t kTmem = HD <= 128 ? 256 : 512, kTmemQ = 64, kTmemO = 64 + HD / 2;
+  static_assert(kTmemO + HD <= kTmem, "TMEM");
 };
 
 // A run of tiles of one (job, KV head), as the producer hands it to the consumers.
@@ -226,14 +236,17 @@ template <int HD>
 struct Smem {
   uint8_t kv[Cfg<HD>::kStages][2][Cfg<HD>::kOperand];
   float red[4][4][HD];  // four rows of each warp's partial result
-  uint8_t q[Cfg<HD>::kQSmem ? 64 * Cfg<HD>::kQPitch : 16];
+  uint8_t q[Cfg<HD>::kQSmem ? 16 * Cfg<HD>::kQPitch : 16];
   int scan[kMaxJobs + 1];
   int ids[kMaxPre];     // prefix jobs: group and block
   Run run[kRuns];
   float mw[4][16], lw[4][16];
   uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages], run_full[kRuns];
+  uint64_t s_full[2], o_full[2];  // tcgen05, a half tile: S = Q K^T, O += P V done
+  uint64_t q_full, p_full[2];     // Q, P in TMEM (each consumer warp)
+  uint32_t tmem;
   int bad[Cfg<HD>::kStages];  // 16-position blocks of the stage without a page
-  int max_cost, abort_flag;
+  int abort_flag;
 };
 static_assert(sizeof(Smem<128>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 128");
 static_assert(sizeof(Smem<64>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 64");
@@ -241,7 +254,7 @@ static_assert(sizeof(Smem<256>) <= 227 * 1024, "shared memory at hd 256");
 // the ring doubles as scratch while the job list is built: row lengths, group boundaries, prefixes
 static_assert((kMaxRows + 2 * kMaxPre + 1) * sizeof(int) <= 6 * 2 * kTile * 64 * 2, "scratch");
 
-// The job list: scan[j] = cost of the jobs before j (per KV head), own jobs first.  All threads of the
+// The job list: scan[j] = tiles of the jobs before j (per KV head), own jobs first.  All threads of the
 // CTA; everything it needs from memory is requested first, in one go.  Returns whether the groups
 // are unusable (their boundaries do not ascend inside the batch: reported, nobody shares anything).
 template <int HD>
@@ -261,14 +274,8 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
   }
   for (int r = tid; r < P.R; r += kThreads) len[r] = row_len(P, r);
   for (int j = n_own + tid; j < n_jobs; j += kThreads) sm.scan[j] = 0;
-  if (tid == 0) sm.max_cost = 1;
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) report_error(P.err, HM_ERR_BADINDEX);
-  auto put = [&](int j, const Job& J) {
-    const int c = tile_cost(J.mt), t = tiles_of(J);
-    if (t && c > 1) atomicMax(&sm.max_cost, c);
-    sm.scan[j] = t * c;
-  };
   // eight lanes share a job's rows (one where a block is one row)
   const bool single = P.S == 1 && P.own_blocks == 1;
   const int step = single ? 1 : 8, mine = tid & (step - 1);
@@ -290,7 +297,7 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
       for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     J.hi = min(J.hi, top);
-    if (j < n_own && mine == 0) put(j, J);
+    if (j < n_own && mine == 0) sm.scan[j] = tiles_of(J);
   }
   // a warp per group, eight lanes per block of its rows
   for (int g = tid >> 5; g < P.n_groups && !bad; g += kThreads / 32) {
@@ -307,7 +314,7 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
       for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       J.hi = min(J.hi, top);
       if (J.M > 0 && (lane & 7) == 0) {
-        put(first + blk, J);
+        sm.scan[first + blk] = tiles_of(J);
         sm.ids[first + blk - n_own] = g | (blk << 16);
       }
     }
@@ -337,8 +344,8 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
   return bad;
 }
 
-// The job whose cost range (scan * Hk + kh * cost + tile * tile_cost) holds x: the last that starts
-// at or before it (jobs without tiles in front of it share its start).
+// The job that holds tile x of the flat order (scan * Hk + kh * tiles + t): the last that starts at or
+// before it (jobs without tiles in front of it share its start).
 HM_DEV int job_at(const int* scan, int n_jobs, int64_t x, int Hk) {
   int lo = 0, hi = n_jobs - 1;
   while (lo < hi) {
@@ -351,7 +358,15 @@ HM_DEV int job_at(const int* scan, int n_jobs, int64_t x, int Hk) {
   return lo;
 }
 
-// ---------------------------------------------------------------- consumer
+// Byte offset of positions 16 * b .. of a tile in its boxes of 2^shift positions, each
+// [64-dim part][position][128 bytes].
+template <int HD>
+HM_DEV uint32_t block_at(int shift, int b) {
+  const int p = 16 * b;
+  return (static_cast<uint32_t>(p >> shift) << shift) * 128u * (HD / 64) + static_cast<uint32_t>(p & ((1 << shift) - 1)) * 128u;
+}
+
+// ---------------------------------------------------------------- blocks of up to 16 rows
 template <int HD, typename T>
 struct Consumer {
   const Params& P;
@@ -361,7 +376,6 @@ struct Consumer {
   float m[2], l[2];
   int lim[2];  // positions that this lane's two rows see
   uint32_t qf[Cfg<HD>::kQSmem ? 1 : HD / 16][4];
-  int qrow, part;  // first query row and position group of this warp
 
   HM_DEV Consumer(const Params& p, Smem<HD>& s) : P(p), sm(s) {
     warp = threadIdx.x >> 5;
@@ -377,15 +391,12 @@ struct Consumer {
     return reinterpret_cast<const T*>(P.q) + (int64_t)(J.row0 + v / P.G) * P.ld_q + (int64_t)(kh * P.G + v % P.G) * HD;
   }
 
-  // Query fragments, limits and cleared statistics of a run.  NB: row groups of the block (1, 2, 4).
-  template <int NB>
+  // Query fragments, limits and cleared statistics of a run.
   HM_DEV void begin(const Job& J, int kh) {
-    qrow = 16 * (warp & (NB - 1));
-    part = warp / NB;
     int64_t p[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int i = qrow + g + 8 * e;
+      const int i = g + 8 * e;
       p[e] = i < J.M ? row_len(P, J.row0 + (J.i0 + i) / P.G) : J.hi;
       m[e] = -INFINITY;
       l[e] = 0.f;
@@ -394,14 +405,14 @@ struct Consumer {
     for (int n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     if constexpr (Cfg<HD>::kQSmem) {
       named_bar(1, kCons);  // the last run's fragments are no longer read
-      for (int c = threadIdx.x; c < 16 * NB * (HD / 8); c += kCons) {
+      for (int c = threadIdx.x; c < 16 * (HD / 8); c += kCons) {
         const int i = c / (HD / 8), d = c % (HD / 8);
         const uint4 v = i < J.M ? *reinterpret_cast<const uint4*>(q_ptr(J, kh, i) + 8 * d) : make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(sm.q + i * Cfg<HD>::kQPitch + 16 * d) = v;
       }
       named_bar(1, kCons);
     } else {
-      const int i = qrow + g;
+      const int i = g;
       const T* a = q_ptr(J, kh, i < J.M ? i : 0) + 2 * t;
       const T* b = q_ptr(J, kh, i + 8 < J.M ? i + 8 : 0) + 2 * t;
 #pragma unroll
@@ -419,84 +430,43 @@ struct Consumer {
   HM_DEV void q_frag(int ks, uint32_t (&a)[4]) const {
     if constexpr (Cfg<HD>::kQSmem) {
       ldsm_x4(a[0], a[1], a[2], a[3],
-              smem_u32(sm.q + (qrow + (mi & 1) * 8 + ri) * Cfg<HD>::kQPitch + ks * 32 + (mi >> 1) * 16));
+              smem_u32(sm.q + ((mi & 1) * 8 + ri) * Cfg<HD>::kQPitch + ks * 32 + (mi >> 1) * 16));
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) a[e] = qf[ks][e];
     }
   }
 
-  // This warp's 16 * NB positions of a tile from p0 (NB = row groups of the block).
-  template <int NB>
+  // This warp's 16 positions of a tile from p0.
   HM_DEV void tile(int st, int p0, int lo, int hi, int bad) {
-    const int b0 = NB * part;
-    if (p0 + 16 * b0 >= hi || p0 + 16 * (b0 + NB) <= lo) return;
-    const uint32_t kb = smem_u32(sm.kv[st][0]), vb = smem_u32(sm.kv[st][1]);
-    const int sub = 1 << P.sub_shift;                         // positions of a box: [64-dim part][position][128 bytes]
-    const uint32_t half = static_cast<uint32_t>(sub) * 128u;
-    // byte offset of position 16 * b of the tile in its box
-    auto block_at = [&](int b) {
-      const int p = 16 * b;
-      return static_cast<uint32_t>(p >> P.sub_shift) * half * (HD / 64) + static_cast<uint32_t>(p & (sub - 1)) * 128u;
-    };
-    float s[2 * NB][4];
+    const int b0 = p0 + 16 * warp;
+    if (b0 >= hi || b0 + 16 <= lo) return;
+    const uint32_t half = 128u << P.sub_shift;
+    const uint32_t at = block_at<HD>(P.sub_shift, warp), kb = smem_u32(sm.kv[st][0]) + at, vb = smem_u32(sm.kv[st][1]) + at;
+    // two sums a score: half the chain of dependent products
+    float s[2][4] = {}, s2[2][4] = {};
 #pragma unroll
-    for (int n = 0; n < 2 * NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    if constexpr (NB == 1) {  // two sums a score: half the chain of dependent products
-      float s2[2][4] = {};
-      const int row = (mi >= 2 ? 8 : 0) + ri;
-      const uint32_t at = kb + block_at(b0) + row * 128;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t a[4], x0, x1, x2, x3;
-        q_frag(ks, a);
-        const int c = 2 * ks + (mi & 1);
-        ldsm_x4(x0, x1, x2, x3, at + (c >> 3) * half + (((c & 7) ^ ri) << 4));
-        Ty<T>::mma(ks & 1 ? s2[0] : s[0], a, x0, x1);
-        Ty<T>::mma(ks & 1 ? s2[1] : s[1], a, x2, x3);
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
-    } else {
-      const int row = (mi >= 2 ? 8 : 0) + ri;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t a[4];
-        q_frag(ks, a);
-        const int c = 2 * ks + (mi & 1);
-        const uint32_t off = (c >> 3) * half + row * 128 + (((c & 7) ^ ri) << 4);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          uint32_t x0, x1, x2, x3;
-          ldsm_x4(x0, x1, x2, x3, kb + block_at(b0 + b) + off);
-          Ty<T>::mma(s[2 * b], a, x0, x1);
-          Ty<T>::mma(s[2 * b + 1], a, x2, x3);
-        }
-      }
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      uint32_t a[4], x0, x1, x2, x3;
+      q_frag(ks, a);
+      const int c = 2 * ks + (mi & 1);
+      ldsm_x4(x0, x1, x2, x3, kb + (c >> 3) * half + ((mi >= 2 ? 8 : 0) + ri) * 128 + (((c & 7) ^ ri) << 4));
+      Ty<T>::mma(ks & 1 ? s2[0] : s[0], a, x0, x1);
+      Ty<T>::mma(ks & 1 ? s2[1] : s[1], a, x2, x3);
     }
-    const bool edge = p0 < lo || p0 + kTile > hi || bad;  // the same for the whole CTA
+    const bool no = (bad >> warp) & 1;
+    const bool edge = b0 < lo || b0 + 16 > hi || no;  // V rows that are not the job's
+    const bool mask = edge || b0 + 16 > min(lim[0], lim[1]);
     float top[2] = {-INFINITY, -INFINITY};
-    if (edge || p0 + kTile > min(lim[0], lim[1])) {
 #pragma unroll
-      for (int n = 0; n < 2 * NB; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int b = b0 + n / 2, p = p0 + 16 * b + 8 * (n & 1) + 2 * t + (e & 1);
-          const bool ok = p >= lo && p < lim[e >> 1] && !((bad >> b) & 1);
-          s[n][e] = ok ? s[n][e] * P.scale : -INFINITY;
-          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < 2 * NB; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] *= P.scale;
-          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-        }
-    }
+      for (int e = 0; e < 4; ++e) {
+        const int p = b0 + 8 * n + 2 * t + (e & 1);
+        const float x = (s[n][e] + s2[n][e]) * P.scale;
+        s[n][e] = mask && (no || p < lo || p >= lim[e >> 1]) ? -INFINITY : x;
+        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      }
     float alpha[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -510,7 +480,7 @@ struct Consumer {
     }
     float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < 2 * NB; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[n][e] = ex2(s[n][e] - top[e >> 1]);
@@ -527,131 +497,341 @@ struct Consumer {
         acc[n][3] *= alpha[1];
       }
     }
+    const uint32_t a[4] = {Ty<T>::pack(s[0][0], s[0][1]), Ty<T>::pack(s[0][2], s[0][3]), Ty<T>::pack(s[1][0], s[1][1]),
+                           Ty<T>::pack(s[1][2], s[1][3])};
+    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // V rows of this lane that belong to the job
+    if (edge) {
+      const int p = b0 + 2 * t;
+      auto in = [&](int x) { return !no && x >= lo && x < hi; };
+      keep0 = (in(p) ? 0xffffu : 0u) | (in(p + 1) ? 0xffff0000u : 0u);
+      keep1 = (in(p + 8) ? 0xffffu : 0u) | (in(p + 9) ? 0xffff0000u : 0u);
+    }
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const uint32_t a[4] = {Ty<T>::pack(s[2 * b][0], s[2 * b][1]), Ty<T>::pack(s[2 * b][2], s[2 * b][3]),
-                             Ty<T>::pack(s[2 * b + 1][0], s[2 * b + 1][1]), Ty<T>::pack(s[2 * b + 1][2], s[2 * b + 1][3])};
-      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // V rows of this lane that belong to the job
+    for (int nd = 0; nd < HD / 16; ++nd) {
+      const int c = 2 * nd + (mi >> 1);
+      uint32_t v0, v1, v2, v3;
+      ldsm_x4_t(v0, v1, v2, v3, vb + (c >> 3) * half + ((mi & 1) * 8 + ri) * 128 + (((c & 7) ^ ri) << 4));
       if (edge) {
-        const int p = p0 + 16 * (b0 + b) + 2 * t;
-        const bool no = (bad >> (b0 + b)) & 1;
-        auto in = [&](int x) { return !no && x >= lo && x < hi; };
-        keep0 = (in(p) ? 0xffffu : 0u) | (in(p + 1) ? 0xffff0000u : 0u);
-        keep1 = (in(p + 8) ? 0xffffu : 0u) | (in(p + 9) ? 0xffff0000u : 0u);
+        v0 &= keep0;
+        v1 &= keep1;
+        v2 &= keep0;
+        v3 &= keep1;
       }
-      const uint32_t base = vb + block_at(b0 + b);
-      const int row = (mi & 1) * 8 + ri;
-#pragma unroll
-      for (int nd = 0; nd < HD / 16; ++nd) {
-        const int c = 2 * nd + (mi >> 1);
-        uint32_t v0, v1, v2, v3;
-        ldsm_x4_t(v0, v1, v2, v3, base + (c >> 3) * half + row * 128 + (((c & 7) ^ ri) << 4));
-        if (edge) {
-          v0 &= keep0;
-          v1 &= keep1;
-          v2 &= keep0;
-          v3 &= keep1;
-        }
-        Ty<T>::mma(acc[2 * nd], a, v0, v1);
-        Ty<T>::mma(acc[2 * nd + 1], a, v2, v3);
-      }
+      Ty<T>::mma(acc[2 * nd], a, v0, v1);
+      Ty<T>::mma(acc[2 * nd + 1], a, v2, v3);
     }
   }
 
-  // The run's partial result goes to rows row_at .. row_at + M - 1 of the workspace.
-  template <int NB>
+  // The run's partial result goes to rows row_at .. row_at + M - 1 of the workspace: the four warps'
+  // join with their common maximum, four rows at a time.
   HM_DEV void finish(int M, int64_t row_at) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    }
-    if constexpr (NB == 4) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = qrow + g + 8 * e;
-        if (i >= M) continue;
-        float* a = P.pa + (row_at + i) * HD + 2 * t;
-#pragma unroll
-        for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(a + 8 * n) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
-        if (t == 0) {
-          P.pm[row_at + i] = m[e];
-          P.pl[row_at + i] = l[e];
-        }
-      }
-    } else {
-      // the position groups of a row join with their common maximum, four rows of every warp at a time
       if (t == 0) {
+        sm.mw[warp][g + 8 * e] = m[e];
+        sm.lw[warp][g + 8 * e] = l[e];
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sm.mw[warp][g + 8 * e] = m[e];
-          sm.lw[warp][g + 8 * e] = l[e];
+    for (int c = 0; c < 4; ++c) {
+      if (4 * c >= M) break;
+      if (c) named_bar(1, kCons);  // the last four rows have been read
+      if ((g >> 2) == (c & 1)) {
+        const int e = c >> 1;
+        float* a = &sm.red[warp][g & 3][2 * t];
+        if (g + 8 * e < M) {
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(a + 8 * n) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
         }
       }
+      named_bar(1, kCons);
+      // 4 rows x HD / 4 columns of 16 bytes
+      for (int x = threadIdx.x; x < HD; x += kCons) {
+        const int k = x / (HD / 4), i = 4 * c + k, d = 4 * (x % (HD / 4));
+        if (i >= M) continue;
+        const float top = fmaxf(fmaxf(sm.mw[0][i], sm.mw[1][i]), fmaxf(sm.mw[2][i], sm.mw[3][i]));
+        const float top0 = top == -INFINITY ? 0.f : top;
+        float den = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (4 * c >= M) break;
-        if (c) named_bar(1, kCons);  // the last four rows have been read
-        if ((g >> 2) == (c & 1)) {
-          const int e = c >> 1;
-          float* a = &sm.red[warp][g & 3][2 * t];
-          if (qrow + g + 8 * e < M) {
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(a + 8 * n) = make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
-          }
+        for (int w = 0; w < 4; ++w) {
+          const float f = ex2(sm.mw[w][i] - top0);
+          const float4 v = *reinterpret_cast<const float4*>(&sm.red[w][k][d]);
+          y.x += f * v.x;
+          y.y += f * v.y;
+          y.z += f * v.z;
+          y.w += f * v.w;
+          den += f * sm.lw[w][i];
         }
-        named_bar(1, kCons);
-        // NB row groups x 4 rows x HD / 4 columns of 16 bytes
-        for (int x = threadIdx.x; x < NB * HD; x += kCons) {
-          const int rg = x / HD, k = x % HD / (HD / 4), i = 4 * c + k, d = 4 * (x % (HD / 4));
-          if (16 * rg + i >= M) continue;
-          float top = -INFINITY, den = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4 / NB; ++w) top = fmaxf(top, sm.mw[rg + NB * w][i]);
-          const float top0 = top == -INFINITY ? 0.f : top;
-          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < 4 / NB; ++w) {
-            const float f = ex2(sm.mw[rg + NB * w][i] - top0);
-            const float4 v = *reinterpret_cast<const float4*>(&sm.red[rg + NB * w][k][d]);
-            y.x += f * v.x;
-            y.y += f * v.y;
-            y.z += f * v.z;
-            y.w += f * v.w;
-            den += f * sm.lw[rg + NB * w][i];
-          }
-          const int64_t row = row_at + 16 * rg + i;
-          *reinterpret_cast<float4*>(P.pa + row * HD + d) = y;
-          if (d == 0) {
-            P.pm[row] = top;
-            P.pl[row] = den;
-          }
+        *reinterpret_cast<float4*>(P.pa + (row_at + i) * HD + d) = y;
+        if (d == 0) {
+          P.pm[row_at + i] = top;
+          P.pl[row_at + i] = den;
         }
       }
     }
   }
 };
 
+template <int HD>
+HM_DEV void advance(int& st, int& ph) {
+  if (++st == Cfg<HD>::kStages) {
+    st = 0;
+    ph ^= 1;
+  }
+}
+
+// First workspace row of a run's partial result.
+HM_DEV int64_t run_row(const Params& P, const Run& run) {
+  return run.prefix ? (int64_t)run.slot * P.pre_rows : P.pre_slots * P.pre_rows + (int64_t)run.slot * P.own_rows;
+}
+
 // A run: its query rows first (the tiles are on their way), then all of its tiles.
-template <int HD, typename T, int NB>
+template <int HD, typename T>
 HM_DEV void consume(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph) {
   Consumer<HD, T> C(P, sm);
   const Job J = run.J;
-  const int64_t row_at = run.prefix ? (int64_t)run.slot * P.pre_rows : P.pre_slots * P.pre_rows + (int64_t)run.slot * P.own_rows;
+  const int64_t row_at = run_row(P, run);
   int left = run.tiles, p0 = run.tile * kTile;
-  C.template begin<NB>(J, run.kh);
+  C.begin(J, run.kh);
   for (; left > 0; --left, p0 += kTile) {
     // on a timeout: carry on, the error is flagged (every warp has to reach finish's barriers)
     mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
-    C.template tile<NB>(st, p0, J.lo, J.hi, sm.bad[st]);
+    C.tile(st, p0, J.lo, J.hi, sm.bad[st]);
     __syncwarp();
     if (C.lane == 0) mbar_arrive(&sm.empty[st]);
-    if (++st == Cfg<HD>::kStages) {
-      st = 0;
-      ph ^= 1;
-    }
+    advance<HD>(st, ph);
   }
-  C.template finish<NB>(J.M, row_at);
+  C.finish(J.M, row_at);
+}
+
+// ---------------------------------------------------------------- blocks of up to 128 rows
+// A tile is two halves of 32 positions whose S (and P over it) have 32 TMEM columns each: while the
+// consumers work on one half, the issuer has the other half's products done.
+//   issuer, half h of tile t: wait for P -> O += P V -> wait for it -> S of half h of tile t + 1.
+constexpr int kHalf = 32;
+
+// S of half h of the tile in stage st.
+template <int HD, typename T>
+HM_DEV void issue_s(const Params& P, Smem<HD>& sm, int st, int h) {
+  const uint32_t half = 128u << P.sub_shift, kb = smem_u32(sm.kv[st][0]);
+  const int sub = min(1 << P.sub_shift, kHalf);  // positions of a box inside this half
+  const uint32_t id = idesc_f16(kBig, 8) - (1u << 17) + (static_cast<uint32_t>(sub >> 3) << 17) + Ty<T>::kFormat;
+  if (elect_one()) {
+    for (int p = 0; p < kHalf; p += sub) {
+      const uint64_t b = sw128_desc(kb + block_at<HD>(P.sub_shift, (kHalf * h + p) / 16));
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        umma_f16_ts(sm.tmem + kHalf * h + p, sm.tmem + Cfg<HD>::kTmemQ + 8 * ks, b + (ks / 4) * (half >> 4) + 2 * (ks % 4), id,
+                    ks != 0);
+    }
+    umma_commit(&sm.s_full[h]);
+  }
+  __syncwarp();
+}
+
+// hph: parity of the halves' barriers (each takes one phase per tile).
+template <int HD, typename T>
+HM_DEV void issue_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& qph, int& hph) {
+  const uint32_t half = 128u << P.sub_shift;
+  constexpr uint32_t id_o = idesc_f16(kBig, HD, false, true) | Ty<T>::kFormat;
+  mbar_wait_short(&sm.q_full, qph, P.err, &sm.abort_flag);
+  qph ^= 1;
+  mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
+  tc_fence_after();
+  issue_s<HD, T>(P, sm, st, 0);
+  issue_s<HD, T>(P, sm, st, 1);
+  for (int t = 0, n = run.tiles; t < n; ++t) {
+    int st2 = st, ph2 = ph;
+    advance<HD>(st2, ph2);
+    const uint32_t vb = smem_u32(sm.kv[st][1]);
+    bool ahead = false;  // the next tile's first S is issued between the halves when its K is there
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mbar_wait_short(&sm.p_full[h], hph, P.err, &sm.abort_flag);
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int b = 0; b < kHalf / 16; ++b)
+          umma_f16_ts(sm.tmem + Cfg<HD>::kTmemO, sm.tmem + kHalf * h + 8 * b,
+                      sw128_mn_desc(vb + block_at<HD>(P.sub_shift, 2 * h + b), half), id_o, (t | h | b) != 0);
+        umma_commit(&sm.o_full[h]);
+      }
+      __syncwarp();
+      mbar_wait_short(&sm.o_full[h], hph, P.err, &sm.abort_flag);
+      tc_fence_after();
+      if (h == 0) {
+        ahead = t + 1 < n && __all_sync(0xffffffffu, mbar_try_wait(&sm.full[st2], ph2));
+        if (ahead) issue_s<HD, T>(P, sm, st2, 0);
+      } else {  // both halves are done with the stage
+        if (elect_one()) mbar_arrive_n(&sm.empty[st], 5);
+        __syncwarp();
+        if (t + 1 < n) {
+          if (!ahead) {
+            mbar_wait_short(&sm.full[st2], ph2, P.err, &sm.abort_flag);
+            issue_s<HD, T>(P, sm, st2, 0);
+          }
+          issue_s<HD, T>(P, sm, st2, 1);
+        }
+      }
+    }
+    hph ^= 1;
+    st = st2;
+    ph = ph2;
+  }
+}
+
+// Consumers: thread = query row of the block = TMEM lane.
+template <int HD, typename T>
+HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& hph) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = threadIdx.x;
+  const Job J = run.J;
+  const int64_t row_at = run_row(P, run);
+  const uint32_t tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16);
+  const bool mine = 32 * warp < J.M;  // whole warps: some rows of this one exist
+  const int v = J.i0 + (i < J.M ? i : 0), r = J.row0 + v / P.G;
+  if (mine) {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + (int64_t)r * P.ld_q +
+                                                    (int64_t)(run.kh * P.G + v % P.G) * HD);
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) {
+      uint32_t x[32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint4 y = i < J.M ? q[8 * c + k] : make_uint4(0, 0, 0, 0);
+        x[4 * k] = y.x;
+        x[4 * k + 1] = y.y;
+        x[4 * k + 2] = y.z;
+        x[4 * k + 3] = y.w;
+      }
+      __syncwarp();
+      tmem_st32(tmem + Cfg<HD>::kTmemQ + 32 * c, x);
+    }
+    tmem_wait_st();
+  }
+  auto publish = [&](uint64_t* bar) {  // Q or P of this warp's rows
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  publish(&sm.q_full);
+  const int lim = i < J.M ? min(row_len(P, r), J.hi) : 0;
+  float m = 0.f, l = 0.f;  // m: the row's reference, at most 2^8 behind its maximum
+  bool seen = false;
+  for (int t = 0, n = run.tiles, p0 = run.tile * kTile; t < n; ++t, p0 += kTile) {
+    mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
+    const int bad = sm.bad[st];
+    if (p0 < J.lo || p0 + kTile > J.hi) {
+      // V rows that are not the job's: zero times whatever stands there must be zero
+      const int p = i >> 1;
+      if (p0 + p < J.lo || p0 + p >= J.hi) {
+        uint8_t* row = sm.kv[st][1] + block_at<HD>(P.sub_shift, p >> 4) + (p & 15) * 128 + (i & 1) * 64;
+        const uint32_t half = 128u << P.sub_shift;
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(row + h * half + 16 * k) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+    }
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      const int a0 = p0 + kHalf * h;
+      mbar_wait_short(&sm.s_full[h], hph, P.err, &sm.abort_flag);
+      tc_fence_after();
+      __syncwarp();
+      if (mine) {
+        uint32_t x[32];
+        tmem_ld32_nowait(tmem + kHalf * h, x);
+        // the columns that this row sees, a bit each
+        const int from = max(J.lo - a0, 0), to = min(lim - a0, kHalf);
+        uint32_t sees = to > from ? (0xffffffffu >> (kHalf - (to - from))) << from : 0u;
+        if (bad) sees &= ((bad >> (2 * h)) & 1 ? 0xffff0000u : 0xffffffffu) & ((bad >> (2 * h)) & 2 ? 0xffffu : 0xffffffffu);
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, sees != 0xffffffffu && sees != 0u)) {
+#pragma unroll
+          for (int c = 0; c < kHalf; ++c)
+            if (!((sees >> c) & 1)) x[c] = 0xff800000u;  // -infinity
+        }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kHalf; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(x[c]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale;
+        if (sees == 0u) top = -INFINITY;
+        bool grow = false;
+        if (!seen) {  // the first positions that this row sees: nothing in O or l but zeros
+          if (top > -INFINITY) {
+            m = top;
+            seen = true;
+          }
+        } else {
+          grow = top > m + 8.f;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          // O at rest: the product before this half's (of the other half) has to be over
+          mbar_wait_short(&sm.o_full[h ^ 1], h ? hph : hph ^ 1, P.err, &sm.abort_flag);
+          tc_fence_after();
+          const float f = grow ? ex2(m - top) : 1.f;
+          if (grow) m = top;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_ld32_nowait(tmem + Cfg<HD>::kTmemO + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st32(tmem + Cfg<HD>::kTmemO + 32 * c, o);
+          }
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kHalf / 2; ++c) {
+          const float y0 = ex2(fmaf(__uint_as_float(x[2 * c]), P.scale, -m));
+          const float y1 = ex2(fmaf(__uint_as_float(x[2 * c + 1]), P.scale, -m));
+          sum[0] += y0;
+          sum[1] += y1;
+          x[c] = sees ? Ty<T>::pack(y0, y1) : 0u;
+        }
+        if (sees) l += sum[0] + sum[1];
+        __syncwarp();
+        tmem_st16(tmem + kHalf * h, x);
+        tmem_wait_st();
+      }
+      publish(&sm.p_full[h]);
+    }
+    hph ^= 1;
+    advance<HD>(st, ph);
+  }
+  // both halves' last products
+  mbar_wait_short(&sm.o_full[0], hph ^ 1, P.err, &sm.abort_flag);
+  mbar_wait_short(&sm.o_full[1], hph ^ 1, P.err, &sm.abort_flag);
+  tc_fence_after();
+  __syncwarp();
+  if (mine) {
+    if (i < J.M) {
+      P.pm[row_at + i] = seen ? m : -INFINITY;
+      P.pl[row_at + i] = l;
+    }
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld32_nowait(tmem + Cfg<HD>::kTmemO + 32 * c, o);
+      tmem_wait_ld();
+      if (i < J.M) {
+        float4* y = reinterpret_cast<float4*>(P.pa + (row_at + i) * HD + 32 * c);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          y[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
+                             __uint_as_float(o[4 * k + 3]));
+      }
+    }
+    tc_fence_before();
+  }
 }
 
 // ---------------------------------------------------------------- kernel
@@ -673,18 +853,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     sm.abort_flag = 0;
     for (int i = 0; i < NST; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 4);
+      mbar_init(&sm.empty[i], 5);  // the consumer warps and the issuer
     }
     for (int i = 0; i < kRuns; ++i) mbar_init(&sm.run_full[i], 1);
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&sm.s_full[h], 1);
+      mbar_init(&sm.o_full[h], 1);
+      mbar_init(&sm.p_full[h], 4);
+    }
+    mbar_init(&sm.q_full, 4);
     fence_barrier_init();
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  const bool no_groups = build_jobs(P, sm);
+  if (P.big && tid >= kThreads - 32) tmem_alloc(&sm.tmem, Cfg<HD>::kTmem);
+  tc_fence_before();
+  const bool no_groups = build_jobs(P, sm);  // (synchronises the CTA)
+  tc_fence_after();
   const int n_jobs = P.n_jobs, n_own = P.B * P.own_blocks, Hk = P.Hk;
   const int64_t total = (int64_t)sm.scan[n_jobs] * Hk;
-  // at least one tile of every kind: each CTA between a unit's first and last has one of its tiles
-  const int64_t even = (total + gridDim.x - 1) / gridDim.x, share = even > sm.max_cost ? even : sm.max_cost;
+  const int64_t share = total > 0 ? (total + gridDim.x - 1) / gridDim.x : 1;
   if (blockIdx.x == 0) {  // for the join
     if (tid == 0) {
       P.plan[0] = static_cast<int>(share);
@@ -693,7 +881,25 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     for (int j = tid; j <= n_jobs; j += kThreads) P.plan[kPlanScan + j] = sm.scan[j];
   }
 
-  if (tid >= kCons) {
+  if (tid >= kThreads - 32) {
+    // ------------------------------------------------------------ tcgen05 issuer
+    int st = 0, ph = 0, qph = 0, hph = 0;
+    for (int n = 0;; ++n) {
+      if (!mbar_wait_short(&sm.run_full[n % kRuns], (n / kRuns) & 1, P.err, &sm.abort_flag)) break;
+      const Run& run = sm.run[n % kRuns];
+      if (run.tiles == 0) break;
+      if (run.J.mt > 16) {
+        issue_big<HD, T>(P, sm, run, st, ph, qph, hph);
+      } else {  // follow the ring, so that an entry is not overwritten before this warp has read it
+        for (int t = 0, k = run.tiles; t < k; ++t) {
+          mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
+          if (lane == 0) mbar_arrive(&sm.empty[st]);
+          __syncwarp();
+          advance<HD>(st, ph);
+        }
+      }
+    }
+  } else if (tid >= kCons) {
     // ------------------------------------------------------------ producer warp
     const int64_t x0 = share * blockIdx.x, x1 = min(total, x0 + share);
     const int sub = 1 << P.sub_shift, nsub = kTile >> P.sub_shift;
@@ -712,12 +918,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     int j = x0 < x1 ? job_at(sm.scan, n_jobs, x0, Hk) : n_jobs;
     int64_t base = x0 < x1 ? (int64_t)sm.scan[j] * Hk : x1;  // where the unit (j, kh) starts
     for (; base < x1 && go; ++j) {
-      const int cost = sm.scan[j + 1] - sm.scan[j];
-      if (cost == 0) continue;
+      const int tiles = sm.scan[j + 1] - sm.scan[j];
+      if (tiles == 0) continue;
       int kh = 0;
       if (base < x0) {  // the first job: the unit that holds x0
-        kh = static_cast<int>((x0 - base) / cost);
-        base += (int64_t)kh * cost;
+        kh = static_cast<int>((x0 - base) / tiles);
+        base += (int64_t)kh * tiles;
       }
       Job J;
       if (j < n_own) {
@@ -729,7 +935,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
         J = prefix_job(P, id >> 16, P.gstart[g], P.gstart[g + 1], P.plen[g]);
         J.trow = P.owner[g];
       }
-      const int c = tile_cost(J.mt), tiles = cost / c;
       // the job's tiles are known, so hi only has to be exact inside the last one
       int top = 0;
       for (int r = row_first(P, J) + lane; r <= row_last(P, J); r += 32) top = max(top, row_len(P, r));
@@ -737,11 +942,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       const int first = J.lo / kTile;
       const int* const trow = P.table + J.trow * P.table_ld;
       int have = -1, pg = 0, at = 0, bad = 0;  // the batch whose pages the lanes hold
-      for (; kh < Hk && base < x1 && go; ++kh, base += cost) {
-        const int t0 = base < x0 ? static_cast<int>((x0 - base + c - 1) / c) : 0;
-        const int t1 = x1 - base >= cost ? tiles : static_cast<int>((x1 - base + c - 1) / c);
-        if (t0 >= t1) continue;  // the share starts behind the unit's last tile's start
-        // a run is one (job, KV head) of one CTA: along the cost order either grows, so their
+      for (; kh < Hk && base < x1 && go; ++kh, base += tiles) {
+        const int t0 = base < x0 ? static_cast<int>(x0 - base) : 0;
+        const int t1 = x1 - base >= tiles ? tiles : static_cast<int>(x1 - base);
+        // a run is one (job, KV head) of one CTA: along the flat order either grows, so their
         // sum numbers the runs of a kind without collisions
         hand_over(Run{J, kh, first + t0, t1 - t0, (j < n_own ? j : j - n_own) * Hk + kh + static_cast<int>(blockIdx.x),
                       j >= n_own});
@@ -796,20 +1000,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     hand_over(Run{});  // no tiles: the end
   } else {
     // ------------------------------------------------------------ consumers
-    int st = 0, ph = 0;
+    int st = 0, ph = 0, hph = 0;
     for (int n = 0;; ++n) {
       const bool ok = mbar_wait_short(&sm.run_full[n % kRuns], (n / kRuns) & 1, P.err, &sm.abort_flag);
       // after a timeout (flagged) all four warps stop together: none waits for another at a barrier
       if (named_bar_or(1, kCons, !ok)) break;
       const Run& run = sm.run[n % kRuns];
       if (run.tiles == 0) break;
-      if (run.J.mt == 16)
-        consume<HD, T, 1>(P, sm, run, st, ph);
-      else if (run.J.mt == 32)
-        consume<HD, T, 2>(P, sm, run, st, ph);
+      if (run.J.mt > 16)
+        consume_big<HD, T>(P, sm, run, st, ph, hph);
       else
-        consume<HD, T, 4>(P, sm, run, st, ph);
+        consume<HD, T>(P, sm, run, st, ph);
     }
+  }
+  __syncthreads();
+  if (P.big && tid >= kThreads - 32) {
+    tc_fence_after();
+    tmem_dealloc(sm.tmem, Cfg<HD>::kTmem);
   }
 }
 
@@ -839,17 +1046,17 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
   if (P.plan[1]) g = -1;
   int64_t at[2] = {0, 0};  // workspace row of the first split; the next one is a slot further
   int cnt[2] = {0, 0};
-  auto splits = [&](int j, int unit, int row, int c, int kind) {
-    const int s0 = scan[j], cost = scan[j + 1] - s0;
-    if (cost == 0) return;
-    const int64_t x = (int64_t)s0 * P.Hk + (int64_t)kh * cost;
-    const int64_t c0 = x / share, c1 = (x + cost - c) / share;
+  auto splits = [&](int j, int unit, int row, int kind) {
+    const int s0 = scan[j], tiles = scan[j + 1] - s0;
+    if (tiles == 0) return;
+    const int64_t x = (int64_t)s0 * P.Hk + (int64_t)kh * tiles;
+    const int64_t c0 = x / share, c1 = (x + tiles - 1) / share;
     cnt[kind] = static_cast<int>(c1 - c0) + 1;
     at[kind] = ((int64_t)unit * P.Hk + kh + c0) * (kind ? P.pre_rows : P.own_rows) + row +
                (kind ? 0 : P.pre_slots * P.pre_rows);
   };
-  splits(u, u, oi % omt, tile_cost(omt), 0);
-  if (g >= 0) splits(j, j - P.B * P.own_blocks, i % mt, tile_cost(mt), 1);
+  splits(u, u, oi % omt, 0);
+  if (g >= 0) splits(j, j - P.B * P.own_blocks, i % mt, 1);
   const int n = cnt[0] + cnt[1];
   auto row_of = [&](int s) {
     return s < cnt[0] ? at[0] + (int64_t)s * P.own_rows : at[1] + (int64_t)(s - cnt[0]) * P.pre_rows;
@@ -915,7 +1122,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
 
 // ---------------------------------------------------------------- host side
 struct Shape {
-  int B, G, own_blocks, own_rows, pre_rows;
+  int B, G, own_blocks, own_rows, pre_rows, big;
   int64_t pre_jobs, pre_slots, rows;
 };
 
@@ -926,12 +1133,13 @@ bool shape_of(int R, int S, int Hq, int Hk, int n_groups, int ctas, Shape* s) {
   s->G = Hq / Hk;
   if (s->G > 64 || R > kMaxRows) return false;
   const int64_t own = (int64_t)S * s->G, all = (int64_t)R * s->G;
-  const int own_mt = block_rows(static_cast<int>(own > 64 ? 64 : own));
+  const int own_mt = own <= 16 ? 16 : kBig;
   s->own_blocks = static_cast<int>((own + own_mt - 1) / own_mt);
   s->own_rows = static_cast<int>(own < own_mt ? own : own_mt);
-  s->pre_rows = static_cast<int>(all < 64 ? all : 64);
-  // groups of up to 64 rows are one job, larger ones one per started 64 rows
-  s->pre_jobs = n_groups == 0 ? 0 : all / 64 + n_groups;
+  s->pre_rows = static_cast<int>(all < kBig ? all : kBig);
+  // groups of up to 128 rows are one job, larger ones one per started 128 rows
+  s->pre_jobs = n_groups == 0 ? 0 : all / kBig + n_groups;
+  s->big = own > 16 || (n_groups > 0 && all > 16);
   if (s->pre_jobs + (int64_t)s->B * s->own_blocks > kMaxJobs || s->pre_jobs > kMaxPre) return false;
   s->pre_slots = s->pre_jobs ? s->pre_jobs * Hk + ctas : 0;
   s->rows = s->pre_slots * s->pre_rows + ((int64_t)s->B * s->own_blocks * Hk + ctas) * s->own_rows;
@@ -1006,14 +1214,15 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
     return HM_EARG;
   if ((d->dtype != HM_DT_F16 && d->dtype != HM_DT_BF16) || (d->hd != 64 && d->hd != 128 && d->hd != 256)) return HM_EARG;
   if (d->n_groups > 0 && (!d->gstart || !d->owner || !d->plen)) return HM_EARG;
+  if (!(d->scale > 0.f) || !(d->scale < INFINITY)) return HM_EARG;
   const int pg = d->page;
   if (!(pg == 16 || pg == 32 || (pg >= 64 && pg % 64 == 0))) return HM_EARG;
   if (d->n_pages < 1 || d->max_pages < 1 || d->n_table < 1 || d->table_ld < d->max_pages || d->Hk < 1) return HM_EARG;
   // pool rows and positions are 32-bit TMA coordinates / lengths
   if ((int64_t)d->n_pages * d->Hk * pg > 0x7fffff00 || (int64_t)d->max_pages * pg > 0x7fffff00) return HM_EARG;
   if (d->ld_q % 8 || d->ld_o % 8 || d->ld_q < (int64_t)d->Hq * d->hd || d->ld_o < (int64_t)d->Hq * d->hd) return HM_EARG;
-  // costs are 32-bit
-  if (((int64_t)d->max_pages * pg / kTile + 1) * tile_cost(64) * kMaxJobs > 0x7fffffff) return HM_EARG;
+  // tile offsets are 32-bit
+  if (((int64_t)d->max_pages * pg / kTile + 1) * kMaxJobs > 0x7fffffff) return HM_EARG;
   // before anything asks for the device: the sizes do not depend on the number of SMs
   Shape s;
   if (!shape_of(d->R, d->S, d->Hq, d->Hk, d->n_groups, 1, &s)) return HM_EARG;
@@ -1058,6 +1267,7 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
   p.own_blocks = s.own_blocks;
   p.own_rows = s.own_rows;
   p.pre_rows = s.pre_rows;
+  p.big = s.big;
   p.pre_slots = s.pre_slots;
   p.plan = reinterpret_cast<int*>(d->ws);
   p.pa = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(d->ws) + kPlanBytes);

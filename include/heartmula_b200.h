@@ -216,8 +216,9 @@ int hm_decode_attn_noalloc(const void* q, const void* kc, const void* vc, const 
  * owner[g].  Sequences outside every group (n_groups may be 0) read all their own pages.
  * pos[r] < 0: a padding row, o = 0.  A bad position, table row, page or group entry sets
  * HM_ERR_BADINDEX; positions without a page, and rows with a bad position, are left out.
- * hd 64, 128 or 256; page 16, 32 or a multiple of 64; Hq / Hk <= 64; dtype HM_DT_F16 or
- * HM_DT_BF16 (q, k, v, o); at most 1024 row blocks: R*G/64 + n_groups + R/S * ceil(S*G / 64).
+ * hd 64, 128 or 256; page 16, 32 or a multiple of 64; Hq / Hk <= 64; scale > 0; dtype HM_DT_F16 or
+ * HM_DT_BF16 (q, k, v, o); at most 16384 rows and 1024 row blocks: R*G/128 + n_groups (of these at
+ * most 896) + R/S * ceil(S*G / 128).
  * ws: hm_prefix_attn_workspace_bytes(..., sms = hm_device_sm_count), 16-byte aligned, not shared by calls that
  * overlap on the GPU. */
 typedef struct {

@@ -80,6 +80,7 @@ def test_prefix_attn(lib):
                dict(ld_q=1000), dict(ld_o=1016), dict(dtype=0), dict(R=0), dict(S=0), dict(S=3), dict(Hq=7), dict(Hk=0),
                dict(Hk=16), dict(hd=96), dict(n_table=3), dict(max_pages=0), dict(table_ld=7), dict(n_pages=0),
                dict(page=8), dict(page=24), dict(page=96), dict(n_groups=-1), dict(n_groups=1025), dict(R=1025, n_table=2000),
+               dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
                dict(n_pages=1 << 26), dict(max_pages=1 << 26, table_ld=1 << 26), dict(max_pages=1 << 22, table_ld=1 << 22)):
         assert lib.hm_prefix_attn(C.byref(PrefixAttnDesc(**{**good, **kw})), None) == -1, kw
     assert lib.hm_prefix_attn(None, None) == -1

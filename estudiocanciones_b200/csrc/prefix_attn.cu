@@ -46,7 +46,7 @@ namespace {
 
 constexpr int kTile = 64;       // positions per tile
 constexpr int kMaxJobs = 1024;  // jobs of a call (the list lives in shared memory)
-constexpr int kMaxPre = 896;    // prefix jobs, and groups, of a call
+constexpr int kMaxPre = 640;    // prefix jobs, and groups, of a call
 constexpr int kMaxRows = 16384; // query rows of a call
 constexpr int kThreads = 192;   // 4 consumer warps, the producer, the tcgen05 issuer
 constexpr int kCons = 128;
@@ -240,7 +240,7 @@ struct Smem {
   int scan[kMaxJobs + 1];
   int ids[kMaxPre];     // prefix jobs: group and block
   Run run[kRuns];
-  float mw[4][16], lw[4][16];
+  float mw[4][32], lw[4][32];
   uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages], run_full[kRuns];
   uint64_t s_full[2], o_full[2];  // tcgen05, a half tile: S = Q K^T, O += P V done
   uint64_t q_full, p_full[2];     // Q, P in TMEM (each consumer warp)
@@ -683,31 +683,70 @@ HM_DEV void issue_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, in
   }
 }
 
-// Consumers: thread = query row of the block = TMEM lane.
-template <int HD, typename T>
+// W columns of this thread's TMEM lane (no wait).
+template <int W>
+HM_DEV void tmem_ld_nowait(uint32_t taddr, uint32_t* r);
+template <>
+HM_DEV void tmem_ld_nowait<32>(uint32_t taddr, uint32_t* r) { tmem_ld32_nowait(taddr, r); }
+template <>
+HM_DEV void tmem_ld_nowait<16>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+template <>
+HM_DEV void tmem_ld_nowait<8>(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+// Consumers: thread = TMEM lane.  A block of at most 128 / PARTS rows stands PARTS times in the lanes,
+// and copy p does the softmax of columns p * 32 / PARTS .. of every half, its P zero elsewhere: all
+// four warps work (on few rows one warp's exponentials would set the pace), and the copies' O, m
+// and l join at the end.
+template <int HD, typename T, int PARTS>
 HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& hph) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = threadIdx.x;
+  constexpr int NW = 4 / PARTS, W = kHalf / PARTS;  // warps per copy, columns of a half per thread
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rg = warp % NW, part = warp / NW, i = 32 * rg + lane;  // row of the block
   const Job J = run.J;
   const int64_t row_at = run_row(P, run);
   const uint32_t tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16);
-  const bool mine = 32 * warp < J.M;  // whole warps: some rows of this one exist
-  const int v = J.i0 + (i < J.M ? i : 0), r = J.row0 + v / P.G;
+  const bool mine = 32 * rg < J.M;  // whole warps: some rows of this one exist
+  auto q_row = [&](int k) {         // of row k of this warp's 32 (clamped)
+    const int v = J.i0 + min(32 * rg + k, J.M - 1);
+    return reinterpret_cast<const T*>(P.q) + (int64_t)(J.row0 + v / P.G) * P.ld_q + (int64_t)(run.kh * P.G + v % P.G) * HD;
+  };
   if (mine) {
-    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + (int64_t)r * P.ld_q +
-                                                    (int64_t)(run.kh * P.G + v % P.G) * HD);
+    // Q: 32 rows x 64 bytes at a time through shared memory (four lanes a row, whole sectors), then
+    // a row per lane into TMEM
+    uint4 y[HD / 32][4];
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
-      uint32_t x[32];
+    for (int j = 0; j < 4; ++j) {
+      const uint4* q = reinterpret_cast<const uint4*>(q_row(8 * j + (lane >> 2))) + (lane & 3);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint4 y = i < J.M ? q[8 * c + k] : make_uint4(0, 0, 0, 0);
-        x[4 * k] = y.x;
-        x[4 * k + 1] = y.y;
-        x[4 * k + 2] = y.z;
-        x[4 * k + 3] = y.w;
-      }
+      for (int c = 0; c < HD / 32; ++c) y[c][j] = q[4 * c];
+    }
+    uint4* const buf = reinterpret_cast<uint4*>(&sm.red[0][0][0]) + 128 * warp;  // 2 KB of the 8 (or more)
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) {
       __syncwarp();
-      tmem_st32(tmem + Cfg<HD>::kTmemQ + 32 * c, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) buf[(8 * j + (lane >> 2)) * 4 + ((lane & 3) ^ (lane >> 3))] = y[c][j];
+      __syncwarp();
+      uint32_t x[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 z = buf[lane * 4 + (k ^ ((lane >> 1) & 3))];
+        x[4 * k] = z.x;
+        x[4 * k + 1] = z.y;
+        x[4 * k + 2] = z.z;
+        x[4 * k + 3] = z.w;
+      }
+      tmem_st16(tmem + Cfg<HD>::kTmemQ + 16 * c, x);
     }
     tmem_wait_st();
   }
@@ -717,7 +756,7 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
     if (lane == 0) mbar_arrive(bar);
   };
   publish(&sm.q_full);
-  const int lim = i < J.M ? min(row_len(P, r), J.hi) : 0;
+  const int lim = i < J.M ? min(row_len(P, J.row0 + (J.i0 + i) / P.G), J.hi) : 0;
   float m = 0.f, l = 0.f;  // m: the row's reference, at most 2^8 behind its maximum
   bool seen = false;
   for (int t = 0, n = run.tiles, p0 = run.tile * kTile; t < n; ++t, p0 += kTile) {
@@ -725,9 +764,9 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
     const int bad = sm.bad[st];
     if (p0 < J.lo || p0 + kTile > J.hi) {
       // V rows that are not the job's: zero times whatever stands there must be zero
-      const int p = i >> 1;
+      const int p = threadIdx.x >> 1;
       if (p0 + p < J.lo || p0 + p >= J.hi) {
-        uint8_t* row = sm.kv[st][1] + block_at<HD>(P.sub_shift, p >> 4) + (p & 15) * 128 + (i & 1) * 64;
+        uint8_t* row = sm.kv[st][1] + block_at<HD>(P.sub_shift, p >> 4) + (p & 15) * 128 + (threadIdx.x & 1) * 64;
         const uint32_t half = 128u << P.sub_shift;
 #pragma unroll
         for (int h = 0; h < HD / 64; ++h)
@@ -743,21 +782,23 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
       tc_fence_after();
       __syncwarp();
       if (mine) {
-        uint32_t x[32];
-        tmem_ld32_nowait(tmem + kHalf * h, x);
-        // the columns that this row sees, a bit each
+        uint32_t x[W];
+        tmem_ld_nowait<W>(tmem + kHalf * h + W * part, x);
+        // the columns that this row sees, a bit each; then this thread's
         const int from = max(J.lo - a0, 0), to = min(lim - a0, kHalf);
         uint32_t sees = to > from ? (0xffffffffu >> (kHalf - (to - from))) << from : 0u;
         if (bad) sees &= ((bad >> (2 * h)) & 1 ? 0xffff0000u : 0xffffffffu) & ((bad >> (2 * h)) & 2 ? 0xffffu : 0xffffffffu);
+        constexpr uint32_t kAll = 0xffffffffu >> (kHalf - W);
+        sees = (sees >> (W * part)) & kAll;
         tmem_wait_ld();
-        if (__any_sync(0xffffffffu, sees != 0xffffffffu && sees != 0u)) {
+        if (__any_sync(0xffffffffu, sees != kAll && sees != 0u)) {
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c)
+          for (int c = 0; c < W; ++c)
             if (!((sees >> c) & 1)) x[c] = 0xff800000u;  // -infinity
         }
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < kHalf; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(x[c]));
+        for (int c = 0; c < W; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(x[c]));
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale;
         if (sees == 0u) top = -INFINITY;
         bool grow = false;
@@ -788,17 +829,20 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
           }
         }
         float sum[2] = {0.f, 0.f};
+        uint32_t y[kHalf / 2];
 #pragma unroll
-        for (int c = 0; c < kHalf / 2; ++c) {
+        for (int c = 0; c < W / 2; ++c) {
           const float y0 = ex2(fmaf(__uint_as_float(x[2 * c]), P.scale, -m));
           const float y1 = ex2(fmaf(__uint_as_float(x[2 * c + 1]), P.scale, -m));
           sum[0] += y0;
           sum[1] += y1;
-          x[c] = sees ? Ty<T>::pack(y0, y1) : 0u;
+          const uint32_t z = sees ? Ty<T>::pack(y0, y1) : 0u;
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) y[p * W / 2 + c] = p == part ? z : 0u;
         }
         if (sees) l += sum[0] + sum[1];
         __syncwarp();
-        tmem_st16(tmem + kHalf * h, x);
+        tmem_st16(tmem + kHalf * h, y);
         tmem_wait_st();
       }
       publish(&sm.p_full[h]);
@@ -810,28 +854,67 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
   mbar_wait_short(&sm.o_full[0], hph ^ 1, P.err, &sm.abort_flag);
   mbar_wait_short(&sm.o_full[1], hph ^ 1, P.err, &sm.abort_flag);
   tc_fence_after();
-  __syncwarp();
-  if (mine) {
-    if (i < J.M) {
-      P.pm[row_at + i] = seen ? m : -INFINITY;
-      P.pl[row_at + i] = l;
-    }
-#pragma unroll 1
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t o[32];
-      __syncwarp();
-      tmem_ld32_nowait(tmem + Cfg<HD>::kTmemO + 32 * c, o);
-      tmem_wait_ld();
-      if (i < J.M) {
-        float4* y = reinterpret_cast<float4*>(P.pa + (row_at + i) * HD + 32 * c);
+  if (!seen) m = -INFINITY;
+  // the copies' l for their common maximum
+  if constexpr (PARTS > 1) {
+    sm.mw[warp][lane] = m;
+    sm.lw[warp][lane] = l;
+    named_bar(1, kCons);
+    float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          y[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                             __uint_as_float(o[4 * k + 3]));
-      }
+    for (int p = 0; p < PARTS; ++p) top = fmaxf(top, sm.mw[rg + NW * p][lane]);
+    const float top0 = top == -INFINITY ? 0.f : top;
+    l = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      l += ex2(sm.mw[rg + NW * p][lane] - top0) * sm.lw[rg + NW * p][lane];
     }
-    tc_fence_before();
+    m = top;
   }
+  if (part == 0 && i < J.M) {
+    P.pm[row_at + i] = m;
+    P.pl[row_at + i] = l;
+  }
+  // 16 columns at a time through shared memory, where a lane's row becomes four lanes' (whole sectors)
+  // and the copies add up
+  float4* const buf = reinterpret_cast<float4*>(&sm.red[0][0][0]);
+  const int rl = threadIdx.x >> 2, k4 = threadIdx.x & 3;
+#pragma unroll 1
+  for (int c = 0; c < HD / 16; ++c) {
+    float o[16];
+    __syncwarp();
+    tmem_ld16(tmem + Cfg<HD>::kTmemO + 16 * c, o);
+    if (c) named_bar(1, kCons);  // the last columns have been read
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      buf[threadIdx.x * 4 + (k ^ ((lane >> 1) & 3))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    named_bar(1, kCons);
+#pragma unroll
+    for (int g = 0; g < NW; ++g) {
+      const int row = 32 * g + rl;
+      if (row >= J.M) continue;
+      float4 y = buf[row * 4 + (k4 ^ ((rl >> 1) & 3))];
+      if constexpr (PARTS > 1) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) top = fmaxf(top, sm.mw[g + NW * p][rl]);
+        const float top0 = top == -INFINITY ? 0.f : top;
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const float w = ex2(sm.mw[g + NW * p][rl] - top0);
+          const float4 v = buf[(32 * (g + NW * p) + rl) * 4 + (k4 ^ ((rl >> 1) & 3))];
+          z.x += w * v.x;
+          z.y += w * v.y;
+          z.z += w * v.z;
+          z.w += w * v.w;
+        }
+        y = z;
+      }
+      *reinterpret_cast<float4*>(P.pa + (row_at + row) * HD + 16 * c + 4 * k4) = y;
+    }
+  }
+  tc_fence_before();
 }
 
 // ---------------------------------------------------------------- kernel
@@ -1007,10 +1090,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       if (named_bar_or(1, kCons, !ok)) break;
       const Run& run = sm.run[n % kRuns];
       if (run.tiles == 0) break;
-      if (run.J.mt > 16)
-        consume_big<HD, T>(P, sm, run, st, ph, hph);
-      else
+      if (run.J.mt == 16)
         consume<HD, T>(P, sm, run, st, ph);
+      else if (run.J.M <= 32)
+        consume_big<HD, T, 4>(P, sm, run, st, ph, hph);
+      else if (run.J.M <= 64)
+        consume_big<HD, T, 2>(P, sm, run, st, ph, hph);
+      else
+        consume_big<HD, T, 1>(P, sm, run, st, ph, hph);
     }
   }
   __syncthreads();
@@ -1020,48 +1107,59 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
   }
 }
 
-// Joins the partial results of a (row, head), one warp each: the sequence's own in order, then the
-// prefix's.  Nothing to join (a padding row): zeros.
-template <int HD, typename T>
+// x / d for x >= 0: the 64-bit quotient only where it is needed (it takes a few hundred cycles).
+HM_DEV int quotient(int64_t x, int d) {
+  return (x >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(d)) : static_cast<int>(x / d);
+}
+
+// Joins the partial results of a (row, head), WPR warps each: the sequence's own in order, then the
+// prefix's, every WPR-th by one warp.  Nothing to join (a padding row): zeros.  The kernel is a chain
+// of memory latencies, so everything that can be is requested at once: the job list's entries, then
+// the maxima, sums and first columns together.  Four warps a pair while all pairs fit the SMs at once
+// (16 x 24 pairs of ~17 splits: 6.6 us shorter than one warp each), one where there are more
+// (64 x 32 pairs of ~8 splits: 5 us shorter than four).
+template <int HD, typename T, int WPR>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params P) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const bool live = id < (int64_t)P.R * P.Hq;
-  const int r = live ? static_cast<int>(id / P.Hq) : 0, h = static_cast<int>(id % P.Hq), kh = h / P.G, b = r / P.S;
+  __shared__ float part_s[WPR == 1 ? 1 : 4][HD];
+  const int warp = (threadIdx.x >> 5) % WPR, lane = threadIdx.x & 31;
+  const unsigned pair = blockIdx.x * (4 / WPR) + (threadIdx.x >> 5) / WPR;
+  const bool live = pair < static_cast<unsigned>(P.R) * P.Hq;
+  const int r = live ? pair / P.Hq : 0, h = pair % P.Hq, kh = h / P.G, b = r / P.S;
   // the call's inputs do not change while it runs: read them while the first kernel still works
+  const int n_own = P.B * P.own_blocks;
   int g = group_of(P.gstart, P.n_groups, b), i = 0, mt = 16, j = 0;
   if (g >= 0 && group_plen(P, g) > 0) {
     const int a = P.gstart[g];
     mt = block_rows((P.gstart[g + 1] - a) * P.S * P.G);
     i = (r - a * P.S) * P.G + h % P.G;
-    j = group_job(P, P.B * P.own_blocks, g, a) + i / mt;
+    j = group_job(P, n_own, g, a) + i / mt;
   } else {
     g = -1;
   }
   const int omt = block_rows(P.S * P.G), oi = (r % P.S) * P.G + h % P.G, u = b * P.own_blocks + oi / omt;
   pdl_wait();
-  if (!live) return;
+  if (WPR == 1 && !live) return;
   const int* scan = P.plan + kPlanScan;
-  const int64_t share = P.plan[0];
-  if (P.plan[1]) g = -1;
-  int64_t at[2] = {0, 0};  // workspace row of the first split; the next one is a slot further
-  int cnt[2] = {0, 0};
-  auto splits = [&](int j, int unit, int row, int kind) {
-    const int s0 = scan[j], tiles = scan[j + 1] - s0;
-    if (tiles == 0) return;
-    const int64_t x = (int64_t)s0 * P.Hk + (int64_t)kh * tiles;
-    const int64_t c0 = x / share, c1 = (x + tiles - 1) / share;
-    cnt[kind] = static_cast<int>(c1 - c0) + 1;
-    at[kind] = ((int64_t)unit * P.Hk + kh + c0) * (kind ? P.pre_rows : P.own_rows) + row +
-               (kind ? 0 : P.pre_slots * P.pre_rows);
-  };
-  splits(u, u, oi % omt, 0);
-  if (g >= 0) splits(j, j - P.B * P.own_blocks, i % mt, 1);
-  const int n = cnt[0] + cnt[1];
-  auto row_of = [&](int s) {
-    return s < cnt[0] ? at[0] + (int64_t)s * P.own_rows : at[1] + (int64_t)(s - cnt[0]) * P.pre_rows;
-  };
-  constexpr int V = HD / 32, E = 4;  // columns of a lane; splits whose columns are requested at once
+  const int share = P.plan[0], bad = P.plan[1], o0 = scan[u], o1 = scan[u + 1];
+  const int p0 = g >= 0 ? scan[j] : 0, p1 = g >= 0 ? scan[j + 1] : 0;
+  // splits of the two jobs, and the workspace row of the first (the next one is a slot further)
+  int cnt0 = 0, cnt1 = 0;
+  int64_t at0 = 0, at1 = 0;
+  if (o1 > o0) {
+    const int64_t x = (int64_t)o0 * P.Hk + (int64_t)kh * (o1 - o0);
+    const int c0 = quotient(x, share);
+    cnt0 = quotient(x + (o1 - o0) - 1, share) - c0 + 1;
+    at0 = P.pre_slots * P.pre_rows + ((int64_t)u * P.Hk + kh + c0) * P.own_rows + oi % omt;
+  }
+  if (p1 > p0 && !bad) {
+    const int64_t x = (int64_t)p0 * P.Hk + (int64_t)kh * (p1 - p0);
+    const int c0 = quotient(x, share);
+    cnt1 = quotient(x + (p1 - p0) - 1, share) - c0 + 1;
+    at1 = ((int64_t)(j - n_own) * P.Hk + kh + c0) * P.pre_rows + i % mt;
+  }
+  const int n = cnt0 + cnt1;
+  auto row_of = [&](int s) { return s < cnt0 ? at0 + (int64_t)s * P.own_rows : at1 + (int64_t)(s - cnt0) * P.pre_rows; };
+  constexpr int V = HD / 32, E = 6;  // columns of a lane; splits of a warp whose columns are requested early
   auto cols = [&](int s, float (&a)[V]) {
     const float* p = P.pa + row_of(s) * HD + V * lane;
 #pragma unroll
@@ -1071,53 +1169,72 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
       a[e + 1] = f.y;
     }
   };
-  float early[E][V];  // before the maxima are known: one latency less
+  float m = -INFINITY, l = 0.f;  // of split `lane`
+  if (lane < n) {
+    const int64_t rw = row_of(lane);
+    m = P.pm[rw];
+    l = P.pl[rw];
+  }
+  float early[E][V];
 #pragma unroll
-  for (int s = 0; s < E; ++s)
-    if (s < n) cols(s, early[s]);
-  float M = -INFINITY;
-  for (int s = lane; s < n; s += 32) M = fmaxf(M, P.pm[row_of(s)]);
+  for (int k = 0; k < E; ++k)
+    if (warp + WPR * k < n) cols(warp + WPR * k, early[k]);
+  float M = m;
+  for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, P.pm[row_of(s)]);
   M = warp_max(M);
   const float M0 = M == -INFINITY ? 0.f : M;
   float num[V] = {};
   float den = 0.f;
   for (int s0 = 0; s0 < n; s0 += 32) {
-    float w = 0.f, ls = 0.f;
-    if (s0 + lane < n) {
-      const int64_t rw = row_of(s0 + lane);
-      w = ex2(P.pm[rw] - M0);
-      ls = P.pl[rw] * w;
+    if (s0) {
+      m = -INFINITY;
+      l = 0.f;
+      if (s0 + lane < n) {
+        const int64_t rw = row_of(s0 + lane);
+        m = P.pm[rw];
+        l = P.pl[rw];
+      }
     }
-    den += warp_sum(ls);
-    const int e = min(32, n - s0);
-    int s = 0;
+    const float w = ex2(m - M0);  // 0 for lanes without a split
+    den += warp_sum(s0 + lane < n ? l * w : 0.f);
+    int s = s0 + warp;
     if (s0 == 0) {
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const float ws = __shfl_sync(0xffffffffu, w, k);
-        if (k < n) {
+      for (int k = 0; k < E; ++k, s += WPR) {
+        const float ws = __shfl_sync(0xffffffffu, w, warp + WPR * k);
+        if (s < n) {
 #pragma unroll
           for (int v = 0; v < V; ++v) num[v] += ws * early[k][v];
         }
       }
-      s = E;
     }
+    const int e = min(s0 + 32, n);
 #pragma unroll 4
-    for (; s < e; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
+    for (; s < e; s += WPR) {
+      const float ws = __shfl_sync(0xffffffffu, w, s - s0);
       float a[V];
-      cols(s0 + s, a);
+      cols(s, a);
 #pragma unroll
       for (int v = 0; v < V; ++v) num[v] += ws * a[v];
     }
   }
   const float inv = 1.f / den;  // NaN stays NaN
-  uint32_t out[V / 2];
+  T* o = reinterpret_cast<T*>(P.o) + r * P.ld_o + (int64_t)h * HD;
+  if constexpr (WPR == 1) {
 #pragma unroll
-  for (int v = 0; v < V; v += 2) out[v / 2] = den == 0.f ? 0u : Ty<T>::pack(num[v] * inv, num[v + 1] * inv);
-  uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(P.o) + r * P.ld_o + (int64_t)h * HD + V * lane);
+    for (int v = 0; v < V; v += 2)
+      *reinterpret_cast<uint32_t*>(o + V * lane + v) = den == 0.f ? 0u : Ty<T>::pack(num[v] * inv, num[v + 1] * inv);
+  } else {
+    static_assert(WPR == 1 || WPR == 4, "the CTA's four warps");
 #pragma unroll
-  for (int v = 0; v < V / 2; ++v) o[v] = out[v];
+    for (int v = 0; v < V; ++v) part_s[warp][V * lane + v] = num[v];
+    __syncthreads();
+    for (int d = 2 * threadIdx.x; d < HD; d += 256) {
+      const float y0 = ((part_s[0][d] + part_s[1][d]) + part_s[2][d]) + part_s[3][d];
+      const float y1 = ((part_s[0][d + 1] + part_s[1][d + 1]) + part_s[2][d + 1]) + part_s[3][d + 1];
+      *reinterpret_cast<uint32_t*>(o + d) = den == 0.f ? 0u : Ty<T>::pack(y0 * inv, y1 * inv);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -1177,7 +1294,8 @@ bool pool_map(const void* p, int64_t rows, int hd, int sub, bool bf16, CUtensorM
 }
 
 template <int HD, typename T>
-cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int dev, cudaStream_t st) {
+cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int sms, int dev,
+                   cudaStream_t st) {
   constexpr size_t smem = sizeof(Smem<HD>);
   static std::atomic<bool> configured[kMaxDevices];
   if (dev >= kMaxDevices || !configured[dev].load()) {
@@ -1188,14 +1306,16 @@ cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p
   }
   cudaError_t e = hm_launch(prefix_attn_kernel<HD, T>, dim3(grid), dim3(kThreads), smem, st, 0, km, vm, p);
   if (e != cudaSuccess) return e;
-  const int64_t warps = (int64_t)p.R * p.Hq;
-  return hm_launch(prefix_join_kernel<HD, T>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, 1, p);
+  const unsigned pairs = static_cast<unsigned>(p.R) * p.Hq;
+  if (pairs <= 4u * sms) return hm_launch(prefix_join_kernel<HD, T, 4>, dim3(pairs), dim3(128), 0, st, 1, p);
+  return hm_launch(prefix_join_kernel<HD, T, 1>, dim3((pairs + 3) / 4), dim3(128), 0, st, 1, p);
 }
 
 template <int HD>
-cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int dev, cudaStream_t st,
-                     bool bf16) {
-  return bf16 ? launch<HD, __nv_bfloat16>(km, vm, p, grid, dev, st) : launch<HD, __half>(km, vm, p, grid, dev, st);
+cudaError_t launch_t(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int sms, int dev,
+                     cudaStream_t st, bool bf16) {
+  return bf16 ? launch<HD, __nv_bfloat16>(km, vm, p, grid, sms, dev, st)
+              : launch<HD, __half>(km, vm, p, grid, sms, dev, st);
 }
 
 bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u); }
@@ -1277,8 +1397,8 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
   // no more CTAs than there can be tiles
   const int64_t most = (s.pre_jobs + (int64_t)s.B * s.own_blocks) * d->Hk * (((int64_t)d->max_pages * pg) / kTile + 1);
   const int grid = static_cast<int>(most < ctas ? most : ctas);
-  e = d->hd == 64    ? launch_t<64>(km, vm, p, grid, dev, stream, bf16)
-      : d->hd == 128 ? launch_t<128>(km, vm, p, grid, dev, stream, bf16)
-                     : launch_t<256>(km, vm, p, grid, dev, stream, bf16);
+  e = d->hd == 64    ? launch_t<64>(km, vm, p, grid, sms, dev, stream, bf16)
+      : d->hd == 128 ? launch_t<128>(km, vm, p, grid, sms, dev, stream, bf16)
+                     : launch_t<256>(km, vm, p, grid, sms, dev, stream, bf16);
   return e == cudaSuccess ? HM_OK : static_cast<int>(e);
 }

@@ -218,7 +218,7 @@ int hm_decode_attn_noalloc(const void* q, const void* kc, const void* vc, const 
  * HM_ERR_BADINDEX; positions without a page, and rows with a bad position, are left out.
  * hd 64, 128 or 256; page 16, 32 or a multiple of 64; Hq / Hk <= 64; scale > 0; dtype HM_DT_F16 or
  * HM_DT_BF16 (q, k, v, o); at most 16384 rows and 1024 row blocks: R*G/128 + n_groups (of these at
- * most 896) + R/S * ceil(S*G / 128).
+ * most 640) + R/S * ceil(S*G / 128).
  * ws: hm_prefix_attn_workspace_bytes(..., sms = hm_device_sm_count), 16-byte aligned, not shared by calls that
  * overlap on the GPU. */
 typedef struct {

@@ -265,7 +265,8 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
   int* const gp = gs + kMaxPre + 1;
   const int n_own = P.B * P.own_blocks, n_jobs = P.n_jobs;
   bool bad = false;
-  for (int g = tid; g < P.n_groups; g += kThreads) {
+  // (rows from the first thread on, groups from the last: on small calls no thread waits twice)
+  for (int g = kThreads - 1 - tid; g < P.n_groups; g += kThreads) {
     const int a = P.gstart[g], b = P.gstart[g + 1];
     gp[g] = group_plen(P, g);
     gs[g] = a;
@@ -299,8 +300,8 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
     J.hi = min(J.hi, top);
     if (j < n_own && mine == 0) sm.scan[j] = tiles_of(J);
   }
-  // a warp per group, eight lanes per block of its rows
-  for (int g = tid >> 5; g < P.n_groups && !bad; g += kThreads / 32) {
+  // a warp per group (the last warp first, see above), eight lanes per block of its rows
+  for (int g = (kThreads - 1 - tid) >> 5; g < P.n_groups && !bad; g += kThreads / 32) {
     const int plen = gp[g], a = gs[g], b = gs[g + 1];
     if (plen == 0) continue;
     const int rows = (b - a) * P.S * P.G, mt = block_rows(rows), first = group_job(P, n_own, g, a);
@@ -1116,8 +1117,8 @@ HM_DEV int quotient(int64_t x, int d) {
 // prefix's, every WPR-th by one warp.  Nothing to join (a padding row): zeros.  The kernel is a chain
 // of memory latencies, so everything that can be is requested at once: the job list's entries, then
 // the maxima, sums and first columns together.  Four warps a pair while all pairs fit the SMs at once
-// (16 x 24 pairs of ~17 splits: 6.6 us shorter than one warp each), one where there are more
-// (64 x 32 pairs of ~8 splits: 5 us shorter than four).
+// (16 x 24 pairs of ~17 splits: 71.8 us a call, 76.5 with one warp each), one where there are more
+// (64 x 32 pairs of ~8 splits: 45.3 us, 48.7 with four).
 template <int HD, typename T, int WPR>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params P) {
   __shared__ float part_s[WPR == 1 ? 1 : 4][HD];

@@ -31,6 +31,12 @@
 //    A 64-row tile took 4500 cycles with mma.sync and one warp per 16 rows.
 //  * A second small kernel joins the partial results of a row in a fixed order (results do not
 //    depend on scheduling) and writes o; its launch overlaps the first kernel's tail.
+//  * A row that ends inside its group's prefix takes no part in it and reads all its pages itself, so
+//    every row of a prefix job sees all of it. Where the rows of one sequence (S > 1) end at different
+//    positions, a V that is not finite must not reach the rows that do not see it (0 * inf): tiles
+//    that some row sees only in part are looked over, and the products of such a V are added row by
+//    row. Calls with one row per sequence run a variant without that code (kSpread): its registers
+//    and instructions cost a call of 16 sequences on long prefixes 11 % although it never ran.
 // Scores, m, l and a are fp32; the probabilities are rounded to the cache's type for the product
 // with V, as the flat decode attention does (l keeps the unrounded sum).  V rows outside a job's
 // range are zeroed (in registers, in shared memory for tcgen05), so whatever stands there (NaN
@@ -90,6 +96,8 @@ struct Ty;
 template <>
 struct Ty<__half> {
   static constexpr uint32_t kFormat = 0;  // of tcgen05 operands A and B
+  static constexpr uint32_t kExp = 0x7c00u;
+  static HM_DEV float2 f2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   static HM_DEV uint32_t pack(float a, float b) { return pack_h2(a, b); }
   static HM_DEV void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -98,6 +106,8 @@ struct Ty<__half> {
 template <>
 struct Ty<__nv_bfloat16> {
   static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
+  static constexpr uint32_t kExp = 0x7f80u;
+  static HM_DEV float2 f2(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
   static HM_DEV uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -109,6 +119,28 @@ struct Ty<__nv_bfloat16> {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
+
+// Whether one of 8 values is an infinity or NaN.
+template <typename T>
+HM_DEV bool odd16(uint4 v) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    odd |= (u[i] & Ty<T>::kExp) == Ty<T>::kExp || ((u[i] >> 16) & Ty<T>::kExp) == Ty<T>::kExp;
+  return odd;
+}
+
+// Whether 64 bytes of each 64-dim part of a V row (from `row`, parts `half` bytes apart) hold an infinity
+// or NaN.  Out of line, like the products of such values below: their registers and instructions stay
+// out of the loops that hardly ever need them.
+template <typename T, int PARTS>
+__device__ __noinline__ bool odd_row(const uint8_t* row, uint32_t half) {
+  bool odd = false;
+  for (int h = 0; h < PARTS; ++h)
+    for (int k = 0; k < 4; ++k) odd |= odd16<T>(*reinterpret_cast<const uint4*>(row + h * half + 16 * k));
+  return odd;
+}
 
 // Barrier over the first `n` threads of the CTA that returns whether any of them passed true.
 HM_DEV bool named_bar_or(int id, int n, bool p) {
@@ -171,39 +203,46 @@ HM_DEV int group_of(const int* gs, int n_groups, int b) {
 }
 
 // One job: query rows i0 .. i0 + M - 1 of `row0` (i -> row row0 + i / G, head kh * G + i % G) over
-// the positions [lo, hi) of table row `trow`.  mt: rows of the block.
+// the positions [lo, hi) of table row `trow`.  mt: rows of the block; plen: the group's prefix.
 struct Job {
-  int row0, i0, M, lo, hi, trow, mt;
+  int row0, i0, M, lo, hi, trow, mt, plen;
 };
 
 // The first prefix job of a group whose sequences start at a: a group of n rows has at most
 // n / 128 + 1 jobs, so these numbers leave room for all of them without a scan.
 HM_DEV int group_job(const Params& P, int n_own, int g, int a) { return n_own + a * P.S * P.G / kBig + g; }
 
-// Block blk of group g's prefix (sequences a .. b - 1), and of sequence b's own positions behind a
-// prefix of lo.  hi is not yet cut to what the rows see.
+// Block blk of a group's prefix (sequences a .. b - 1), and of sequence b's own positions behind it.
+// Their ranges follow from the rows' lengths, see own_range and prefix_range.
 HM_DEV Job prefix_job(const Params& P, int blk, int a, int b, int plen) {
   Job J;
   const int rows = (b - a) * P.S * P.G;
   J.row0 = a * P.S;
-  J.lo = 0;
-  J.hi = plen;
+  J.lo = J.hi = 0;
+  J.plen = plen;
   J.mt = block_rows(rows);
   J.i0 = blk * J.mt;
   J.M = min(J.mt, rows - J.i0);
   return J;
 }
-HM_DEV Job own_job(const Params& P, int blk, int b, int lo) {
+HM_DEV Job own_job(const Params& P, int blk, int b, int plen) {
   Job J;
   const int rows = P.S * P.G;
   J.row0 = b * P.S;
-  J.lo = lo;
-  J.hi = P.max_pages * P.page;
+  J.lo = J.hi = 0;
+  J.plen = plen;
   J.mt = block_rows(rows);
   J.i0 = blk * J.mt;
   J.M = min(J.mt, rows - J.i0);
   return J;
 }
+// top: the largest length of the job's rows, low: the smallest of those above 0 (else INT_MAX).
+HM_DEV void own_range(Job& J, int top, int low) {
+  J.lo = low < J.plen ? 0 : J.plen;  // a row that ends inside the prefix reads its own pages from the start
+  J.hi = top;
+}
+HM_DEV void prefix_range(Job& J, int top) { J.hi = top >= J.plen ? J.plen : 0; }
+HM_DEV int low_of(int len) { return len > 0 ? len : 0x7fffffff; }
 // First and last query row of a job.
 HM_DEV int row_first(const Params& P, const Job& J) { return J.row0 + J.i0 / P.G; }
 HM_DEV int row_last(const Params& P, const Job& J) { return J.row0 + (J.i0 + J.M - 1) / P.G; }
@@ -283,21 +322,24 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
   for (int j0 = 0; j0 < n_own; j0 += kThreads / step) {
     const int j = j0 + tid / step;
     Job J = {};
-    int top = 0;
+    int top = 0, low = 0x7fffffff;
     if (j < n_own) {
       const int b = P.own_blocks == 1 ? j : j / P.own_blocks;
       const int g = bad ? -1 : group_of(gs, P.n_groups, b);
       J = own_job(P, j - b * P.own_blocks, b, g < 0 ? 0 : gp[g]);
-      if (single)
-        top = len[b];
-      else
-        for (int r = row_first(P, J) + mine; r <= row_last(P, J); r += 8) top = max(top, len[r]);
+      for (int r = single ? b : row_first(P, J) + mine, e = single ? b : row_last(P, J); r <= e; r += 8) {
+        top = max(top, len[r]);
+        low = min(low, low_of(len[r]));
+      }
     }
     if (!single) {
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < 8; o <<= 1) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+      }
     }
-    J.hi = min(J.hi, top);
+    own_range(J, top, low);
     if (j < n_own && mine == 0) sm.scan[j] = tiles_of(J);
   }
   // a warp per group (the last warp first, see above), eight lanes per block of its rows
@@ -313,7 +355,7 @@ HM_DEV bool build_jobs(const Params& P, Smem<HD>& sm) {
         for (int r = row_first(P, J) + (lane & 7); r <= row_last(P, J); r += 8) top = max(top, len[r]);
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      J.hi = min(J.hi, top);
+      prefix_range(J, top);
       if (J.M > 0 && (lane & 7) == 0) {
         sm.scan[first + blk] = tiles_of(J);
         sm.ids[first + blk - n_own] = g | (blk << 16);
@@ -367,15 +409,38 @@ HM_DEV uint32_t block_at(int shift, int b) {
   return (static_cast<uint32_t>(p >> shift) << shift) * 128u * (HD / 64) + static_cast<uint32_t>(p & ((1 << shift) - 1)) * 128u;
 }
 
-// ---------------------------------------------------------------- blocks of up to 16 rows
+// A lane's share of acc += P V in the MMA's layout (rows g and g + 8 of w, columns 8 n + 2 t, + 1 of V),
+// over the positions in see0 / see1 only.
 template <int HD, typename T>
+__device__ __noinline__ void rows_product(float* acc, const float* w, const uint8_t* v, uint32_t half, uint32_t see0,
+                                          uint32_t see1) {
+  for (int p = 0; p < 16; ++p) {
+    for (int n = 0; n < HD / 8; ++n) {
+      const float2 x =
+          Ty<T>::f2(*reinterpret_cast<const uint32_t*>(v + (n / 8) * half + p * 128 + (((n % 8) ^ (p & 7)) << 4)));
+      if ((see0 >> p) & 1) {
+        acc[4 * n] += w[p] * x.x;
+        acc[4 * n + 1] += w[p] * x.y;
+      }
+      if ((see1 >> p) & 1) {
+        acc[4 * n + 2] += w[128 + p] * x.x;
+        acc[4 * n + 3] += w[128 + p] * x.y;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- blocks of up to 16 rows
+// kSpread: the rows of a sequence (S > 1) may end at different positions.
+template <int HD, typename T, bool kSpread>
 struct Consumer {
   const Params& P;
   Smem<HD>& sm;
   int warp, lane, g, t, mi, ri;
   float acc[HD / 8][4];
   float m[2], l[2];
-  int lim[2];  // positions that this lane's two rows see
+  int low[2], lim[2];  // positions [low, lim) that this lane's two rows see
+  bool mixed;          // not the same for all rows of the job
   uint32_t qf[Cfg<HD>::kQSmem ? 1 : HD / 16][4];
 
   HM_DEV Consumer(const Params& p, Smem<HD>& s) : P(p), sm(s) {
@@ -393,12 +458,12 @@ struct Consumer {
   }
 
   // Query fragments, limits and cleared statistics of a run.
-  HM_DEV void begin(const Job& J, int kh) {
-    int64_t p[2];
+  HM_DEV void begin(const Job& J, int kh, bool prefix) {
+    int len[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = g + 8 * e;
-      p[e] = i < J.M ? row_len(P, J.row0 + (J.i0 + i) / P.G) : J.hi;
+      len[e] = kSpread && i < J.M && !prefix ? row_len(P, J.row0 + (J.i0 + i) / P.G) : J.hi;
       m[e] = -INFINITY;
       l[e] = 0.f;
     }
@@ -424,8 +489,12 @@ struct Consumer {
         qf[ks][3] = i + 8 < J.M ? *reinterpret_cast<const uint32_t*>(b + 16 * ks + 8) : 0u;
       }
     }
-    lim[0] = min(static_cast<int>(p[0]), J.hi);
-    lim[1] = min(static_cast<int>(p[1]), J.hi);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      low[e] = kSpread && g + 8 * e < J.M && len[e] >= J.plen && !prefix ? max(J.lo, J.plen) : J.lo;
+      lim[e] = min(len[e], J.hi);
+    }
+    mixed = kSpread && __any_sync(0xffffffffu, low[0] != J.lo || low[1] != J.lo || lim[0] != J.hi || lim[1] != J.hi);
   }
 
   HM_DEV void q_frag(int ks, uint32_t (&a)[4]) const {
@@ -457,7 +526,7 @@ struct Consumer {
     }
     const bool no = (bad >> warp) & 1;
     const bool edge = b0 < lo || b0 + 16 > hi || no;  // V rows that are not the job's
-    const bool mask = edge || b0 + 16 > min(lim[0], lim[1]);
+    const bool mask = edge || (kSpread && mixed);
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -465,7 +534,7 @@ struct Consumer {
       for (int e = 0; e < 4; ++e) {
         const int p = b0 + 8 * n + 2 * t + (e & 1);
         const float x = (s[n][e] + s2[n][e]) * P.scale;
-        s[n][e] = mask && (no || p < lo || p >= lim[e >> 1]) ? -INFINITY : x;
+        s[n][e] = mask && (no || p < low[e >> 1] || p >= lim[e >> 1]) ? -INFINITY : x;
         top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
       }
     float alpha[2];
@@ -507,6 +576,12 @@ struct Consumer {
       keep0 = (in(p) ? 0xffffu : 0u) | (in(p + 1) ? 0xffff0000u : 0u);
       keep1 = (in(p + 8) ? 0xffffu : 0u) | (in(p + 9) ? 0xffff0000u : 0u);
     }
+    if constexpr (kSpread) {
+      if (mixed && !no && partly_unseen(b0, lo, hi) && not_finite(sm.kv[st][1] + at, b0, lo, hi)) {
+        add_rows(sm.kv[st][1] + at, b0, s);
+        return;
+      }
+    }
 #pragma unroll
     for (int nd = 0; nd < HD / 16; ++nd) {
       const int c = 2 * nd + (mi >> 1);
@@ -521,6 +596,41 @@ struct Consumer {
       Ty<T>::mma(acc[2 * nd], a, v0, v1);
       Ty<T>::mma(acc[2 * nd + 1], a, v2, v3);
     }
+  }
+
+  // Whether some row of the block sees only a part of this warp's positions.
+  HM_DEV bool partly_unseen(int b0, int lo, int hi) const {
+    const int a = max(b0, lo), b = min(b0 + 16, hi);
+    return __any_sync(0xffffffffu, low[0] > a || low[1] > a || lim[0] < b || lim[1] < b);
+  }
+  // Whether V of this warp's positions inside [lo, hi) holds an infinity or NaN.
+  HM_DEV bool not_finite(const uint8_t* v, int b0, int lo, int hi) const {
+    const int p = lane >> 1;
+    const bool in = b0 + p >= lo && b0 + p < hi;
+    return __any_sync(0xffffffffu, in && odd_row<T, HD / 64>(v + p * 128 + (lane & 1) * 64, 128u << P.sub_shift));
+  }
+  // acc += P V with every row's own positions only (weights in s).
+  HM_DEV void add_rows(const uint8_t* v, int b0, const float (&s)[2][4]) {
+    float* const w = &sm.red[warp][0][0];  // 16 rows x 16 positions, 0 where the row does not see
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[(g + 8 * (e >> 1)) * 16 + 8 * n + 2 * t + (e & 1)] = s[n][e];
+    __syncwarp();
+    uint32_t sees[2] = {0u, 0u};
+    for (int p = 0; p < 16; ++p)
+      for (int e = 0; e < 2; ++e) sees[e] |= (b0 + p >= low[e] && b0 + p < lim[e] ? 1u : 0u) << p;
+    float a[HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[n][e] = acc[n][e];
+    rows_product<HD, T>(&a[0][0], w + g * 16, v + 4 * t, 128u << P.sub_shift, sees[0], sees[1]);
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = a[n][e];
+    __syncwarp();
   }
 
   // The run's partial result goes to rows row_at .. row_at + M - 1 of the workspace: the four warps'
@@ -590,13 +700,13 @@ HM_DEV int64_t run_row(const Params& P, const Run& run) {
 }
 
 // A run: its query rows first (the tiles are on their way), then all of its tiles.
-template <int HD, typename T>
+template <int HD, typename T, bool kSpread>
 HM_DEV void consume(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph) {
-  Consumer<HD, T> C(P, sm);
+  Consumer<HD, T, kSpread> C(P, sm);
   const Job J = run.J;
   const int64_t row_at = run_row(P, run);
   int left = run.tiles, p0 = run.tile * kTile;
-  C.begin(J, run.kh);
+  C.begin(J, run.kh, run.prefix);
   for (; left > 0; --left, p0 += kTile) {
     // on a timeout: carry on, the error is flagged (every warp has to reach finish's barriers)
     mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
@@ -634,7 +744,7 @@ HM_DEV void issue_s(const Params& P, Smem<HD>& sm, int st, int h) {
 }
 
 // hph: parity of the halves' barriers (each takes one phase per tile).
-template <int HD, typename T>
+template <int HD, typename T, bool kSpread>
 HM_DEV void issue_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& qph, int& hph) {
   const uint32_t half = 128u << P.sub_shift;
   constexpr uint32_t id_o = idesc_f16(kBig, HD, false, true) | Ty<T>::kFormat;
@@ -657,7 +767,8 @@ HM_DEV void issue_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, in
 #pragma unroll
         for (int b = 0; b < kHalf / 16; ++b)
           umma_f16_ts(sm.tmem + Cfg<HD>::kTmemO, sm.tmem + kHalf * h + 8 * b,
-                      sw128_mn_desc(vb + block_at<HD>(P.sub_shift, 2 * h + b), half), id_o, (t | h | b) != 0);
+                      sw128_mn_desc(vb + block_at<HD>(P.sub_shift, 2 * h + b), half), id_o,
+                      kSpread || (t | h | b) != 0);  // (kSpread: the consumers cleared O)
         umma_commit(&sm.o_full[h]);
       }
       __syncwarp();
@@ -698,17 +809,57 @@ HM_DEV void tmem_ld_nowait<16>(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 template <>
+HM_DEV void tmem_ld_nowait<1>(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(taddr));
+}
+template <>
 HM_DEV void tmem_ld_nowait<8>(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
 
+// O += P V of this thread's row for positions q0 .. q0 + W - 1 of the tile, those in `sees` only.
+// Scores are read back from S.
+template <int HD, typename T, int W>
+__device__ __noinline__ void add_row(const uint8_t* v, int sub_shift, uint32_t tmem, int q0, uint32_t sees, float m,
+                                     float scale) {
+#pragma unroll 1
+  for (int c = 0; c < HD / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32_nowait(tmem + Cfg<HD>::kTmemO + 32 * c, o);
+#pragma unroll 1
+    for (int p = 0; p < W; ++p) {
+      uint32_t x;
+      __syncwarp();
+      tmem_ld_nowait<1>(tmem + q0 + p, &x);
+      tmem_wait_ld();
+      if (!((sees >> p) & 1)) continue;
+      const float w = ex2(fmaf(__uint_as_float(x), scale, -m));
+      const int q = q0 + p;
+      const uint8_t* row = v + block_at<HD>(sub_shift, q >> 4) + (c / 2) * (128u << sub_shift) + (q & 15) * 128;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 y = *reinterpret_cast<const uint4*>(row + (((4 * (c & 1) + k) ^ (q & 7)) << 4));
+        const uint32_t u[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = Ty<T>::f2(u[e]);
+          o[8 * k + 2 * e] = __float_as_uint(__uint_as_float(o[8 * k + 2 * e]) + w * f.x);
+          o[8 * k + 2 * e + 1] = __float_as_uint(__uint_as_float(o[8 * k + 2 * e + 1]) + w * f.y);
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st32(tmem + Cfg<HD>::kTmemO + 32 * c, o);
+  }
+}
+
 // Consumers: thread = TMEM lane.  A block of at most 128 / PARTS rows stands PARTS times in the lanes,
 // and copy p does the softmax of columns p * 32 / PARTS .. of every half, its P zero elsewhere: all
 // four warps work (on few rows one warp's exponentials would set the pace), and the copies' O, m
 // and l join at the end.
-template <int HD, typename T, int PARTS>
+template <int HD, typename T, int PARTS, bool kSpread>
 HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& hph) {
   constexpr int NW = 4 / PARTS, W = kHalf / PARTS;  // warps per copy, columns of a half per thread
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -749,6 +900,10 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
       }
       tmem_st16(tmem + Cfg<HD>::kTmemQ + 16 * c, x);
     }
+    if constexpr (kSpread) {  // O = 0: rows may be added to it before the first product
+      uint32_t z[16] = {};
+      for (int c = 0; c < HD / 16; ++c) tmem_st16(tmem + Cfg<HD>::kTmemO + 16 * c, z);
+    }
     tmem_wait_st();
   }
   auto publish = [&](uint64_t* bar) {  // Q or P of this warp's rows
@@ -757,7 +912,17 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
     if (lane == 0) mbar_arrive(bar);
   };
   publish(&sm.q_full);
-  const int lim = i < J.M ? min(row_len(P, J.row0 + (J.i0 + i) / P.G), J.hi) : 0;
+  // positions [low, lim) that this row sees
+  int low = J.lo, lim = i < J.M ? J.hi : 0;
+  bool mixed = false;  // not the same for all rows of the job
+  if (kSpread && !run.prefix) {
+    if (i < J.M) {
+      const int len = row_len(P, J.row0 + (J.i0 + i) / P.G);
+      if (len >= J.plen) low = max(J.lo, J.plen);
+      lim = min(len, J.hi);
+    }
+    mixed = named_bar_or(1, kCons, i < J.M && (low != J.lo || lim != J.hi));
+  }
   float m = 0.f, l = 0.f;  // m: the row's reference, at most 2^8 behind its maximum
   bool seen = false;
   for (int t = 0, n = run.tiles, p0 = run.tile * kTile; t < n; ++t, p0 += kTile) {
@@ -776,6 +941,13 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
       }
       fence_proxy_async_smem();
     }
+    bool slow = false;  // a V that is not finite, and a row that must not see it
+    if (kSpread && mixed && named_bar_or(1, kCons, i < J.M && (low > max(p0, J.lo) || lim < min(p0 + kTile, J.hi)))) {
+      const int p = threadIdx.x >> 1;
+      const uint8_t* row = sm.kv[st][1] + block_at<HD>(P.sub_shift, p >> 4) + (p & 15) * 128 + (threadIdx.x & 1) * 64;
+      const bool in = p0 + p >= J.lo && p0 + p < J.hi;
+      slow = named_bar_or(1, kCons, in && odd_row<T, HD / 64>(row, 128u << P.sub_shift));
+    }
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
       const int a0 = p0 + kHalf * h;
@@ -786,7 +958,7 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
         uint32_t x[W];
         tmem_ld_nowait<W>(tmem + kHalf * h + W * part, x);
         // the columns that this row sees, a bit each; then this thread's
-        const int from = max(J.lo - a0, 0), to = min(lim - a0, kHalf);
+        const int from = max(low - a0, 0), to = min(lim - a0, kHalf);
         uint32_t sees = to > from ? (0xffffffffu >> (kHalf - (to - from))) << from : 0u;
         if (bad) sees &= ((bad >> (2 * h)) & 1 ? 0xffff0000u : 0xffffffffu) & ((bad >> (2 * h)) & 2 ? 0xffffu : 0xffffffffu);
         constexpr uint32_t kAll = 0xffffffffu >> (kHalf - W);
@@ -843,8 +1015,25 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
         }
         if (sees) l += sum[0] + sum[1];
         __syncwarp();
+        if (kSpread && slow) {
+          mbar_wait_short(&sm.o_full[h ^ 1], h ? hph : hph ^ 1, P.err, &sm.abort_flag);  // O at rest, see above
+          tc_fence_after();
+          add_row<HD, T, W>(sm.kv[st][1], P.sub_shift, tmem, kHalf * h + W * part, sees, m, P.scale);
+#pragma unroll
+          for (int c = 0; c < kHalf / 2; ++c) y[c] = 0u;
+        }
         tmem_st16(tmem + kHalf * h, y);
         tmem_wait_st();
+      }
+      if (kSpread && slow) {  // this half's products are in O: zero times zero for the tensor cores
+        named_bar(1, kCons);
+        const int p = kHalf * h + (threadIdx.x >> 2);
+        uint8_t* row = sm.kv[st][1] + block_at<HD>(P.sub_shift, p >> 4) + (p & 15) * 128 + (threadIdx.x & 3) * 32;
+        for (int k = 0; k < HD / 64; ++k) {
+          *reinterpret_cast<uint4*>(row + k * (128u << P.sub_shift)) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(row + k * (128u << P.sub_shift) + 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
       }
       publish(&sm.p_full[h]);
     }
@@ -919,7 +1108,7 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
 }
 
 // ---------------------------------------------------------------- kernel
-template <int HD, typename T>
+template <int HD, typename T, bool kSpread>
 __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ Params P) {
@@ -973,7 +1162,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       const Run& run = sm.run[n % kRuns];
       if (run.tiles == 0) break;
       if (run.J.mt > 16) {
-        issue_big<HD, T>(P, sm, run, st, ph, qph, hph);
+        issue_big<HD, T, kSpread>(P, sm, run, st, ph, qph, hph);
       } else {  // follow the ring, so that an entry is not overwritten before this warp has read it
         for (int t = 0, k = run.tiles; t < k; ++t) {
           mbar_wait_short(&sm.full[st], ph, P.err, &sm.abort_flag);
@@ -1019,10 +1208,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
         J = prefix_job(P, id >> 16, P.gstart[g], P.gstart[g + 1], P.plen[g]);
         J.trow = P.owner[g];
       }
-      // the job's tiles are known, so hi only has to be exact inside the last one
-      int top = 0;
-      for (int r = row_first(P, J) + lane; r <= row_last(P, J); r += 32) top = max(top, row_len(P, r));
-      J.hi = min(J.hi, __reduce_max_sync(0xffffffffu, top));
+      int top = 0, low = 0x7fffffff;
+      for (int r = row_first(P, J) + lane; r <= row_last(P, J); r += 32) {
+        const int len = row_len(P, r);
+        top = max(top, len);
+        low = min(low, low_of(len));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (j < n_own)
+        own_range(J, top, __reduce_min_sync(0xffffffffu, low));
+      else
+        prefix_range(J, top);
       const int first = J.lo / kTile;
       const int* const trow = P.table + J.trow * P.table_ld;
       int have = -1, pg = 0, at = 0, bad = 0;  // the batch whose pages the lanes hold
@@ -1092,13 +1288,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       const Run& run = sm.run[n % kRuns];
       if (run.tiles == 0) break;
       if (run.J.mt == 16)
-        consume<HD, T>(P, sm, run, st, ph);
+        consume<HD, T, kSpread>(P, sm, run, st, ph);
       else if (run.J.M <= 32)
-        consume_big<HD, T, 4>(P, sm, run, st, ph, hph);
+        consume_big<HD, T, 4, kSpread>(P, sm, run, st, ph, hph);
       else if (run.J.M <= 64)
-        consume_big<HD, T, 2>(P, sm, run, st, ph, hph);
+        consume_big<HD, T, 2, kSpread>(P, sm, run, st, ph, hph);
       else
-        consume_big<HD, T, 1>(P, sm, run, st, ph, hph);
+        consume_big<HD, T, 1, kSpread>(P, sm, run, st, ph, hph);
     }
   }
   __syncthreads();
@@ -1129,7 +1325,9 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
   // the call's inputs do not change while it runs: read them while the first kernel still works
   const int n_own = P.B * P.own_blocks;
   int g = group_of(P.gstart, P.n_groups, b), i = 0, mt = 16, j = 0;
-  if (g >= 0 && group_plen(P, g) > 0) {
+  const int plen = g >= 0 ? group_plen(P, g) : 0;
+  // (a bad boundary may be anything)
+  if (plen > 0 && P.gstart[g] >= 0 && P.gstart[g + 1] <= P.B && row_len(P, r) >= plen) {
     const int a = P.gstart[g];
     mt = block_rows((P.gstart[g + 1] - a) * P.S * P.G);
     i = (r - a * P.S) * P.G + h % P.G;
@@ -1294,18 +1492,24 @@ bool pool_map(const void* p, int64_t rows, int hd, int sub, bool bf16, CUtensorM
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, typename T>
-cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int sms, int dev,
-                   cudaStream_t st) {
+template <int HD, typename T, bool kSpread>
+cudaError_t launch_main(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int dev, cudaStream_t st) {
   constexpr size_t smem = sizeof(Smem<HD>);
   static std::atomic<bool> configured[kMaxDevices];
   if (dev >= kMaxDevices || !configured[dev].load()) {
-    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<HD, T, kSpread>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) configured[dev].store(true);
   }
-  cudaError_t e = hm_launch(prefix_attn_kernel<HD, T>, dim3(grid), dim3(kThreads), smem, st, 0, km, vm, p);
+  return hm_launch(prefix_attn_kernel<HD, T, kSpread>, dim3(grid), dim3(kThreads), smem, st, 0, km, vm, p);
+}
+
+template <int HD, typename T>
+cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int grid, int sms, int dev,
+                   cudaStream_t st) {
+  const cudaError_t e = p.S == 1 ? launch_main<HD, T, false>(km, vm, p, grid, dev, st)
+                                 : launch_main<HD, T, true>(km, vm, p, grid, dev, st);
   if (e != cudaSuccess) return e;
   const unsigned pairs = static_cast<unsigned>(p.R) * p.Hq;
   if (pairs <= 4u * sms) return hm_launch(prefix_join_kernel<HD, T, 4>, dim3(pairs), dim3(128), 0, st, 1, p);

@@ -497,8 +497,8 @@ def prefix_attn(q, k, v, table, pos, gstart=None, owner=None, plen=None, S: int 
     Sequences ``gstart[g] <= b < gstart[g + 1]`` hold the same K and V at positions
     ``[0, plen[g])``, read through table row ``owner[g]`` (``gstart [groups + 1]``, ``owner`` and ``plen
     [groups]`` int32 on the device, so a captured call serves every frame); without groups every
-    sequence reads its own pages.  ``pos[r] < 0`` is a padding row and gives zeros.  Returns ``o``
-    like ``q``."""
+    sequence reads its own pages, as does a row that ends inside the prefix.  ``pos[r] < 0`` is a
+    padding row and gives zeros.  Returns ``o`` like ``q``."""
     idx = _device_of("prefix_attn", q, k, v, table, pos, gstart, owner, plen, o, seqs)
     if q.dim() != 2:
         raise HMError("prefix_attn: q [R, Hq * hd]")

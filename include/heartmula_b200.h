@@ -213,7 +213,9 @@ int hm_decode_attn_noalloc(const void* q, const void* kc, const void* vc, const 
  * in table row seqs[b] (seqs NULL: b), and attends to positions [0, pos[r]] of it; o like q.
  * Sequences gstart[g] .. gstart[g+1] - 1 (gstart: n_groups + 1 ascending values) form group g and
  * hold the same K and V at positions [0, plen[g]): those are read once, through table row
- * owner[g].  Sequences outside every group (n_groups may be 0) read all their own pages.
+ * owner[g].  Sequences outside every group (n_groups may be 0), and rows that end inside the prefix
+ * (pos[r] + 1 < plen[g]), read all their own pages.  What stands in a position that a row does not
+ * attend to has no effect on it, infinities and NaN included.
  * pos[r] < 0: a padding row, o = 0.  A bad position, table row, page or group entry sets
  * HM_ERR_BADINDEX; positions without a page, and rows with a bad position, are left out.
  * hd 64, 128 or 256; page 16, 32 or a multiple of 64; Hq / Hk <= 64; scale > 0; dtype HM_DT_F16 or

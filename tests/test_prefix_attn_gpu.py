@@ -101,6 +101,8 @@ class Case:
         for g in range(len(gs) - 1):
             if gs[g] <= b < gs[g + 1]:
                 pl, ow = int(self.plen[g]), int(self.owner[g])
+        if n < pl:   # ends inside the prefix: reads its own pages
+            pl = 0
         t = self.table.tolist()
         out = []
         for p in range(n):
@@ -251,6 +253,43 @@ def test_infinities_outside_a_rows_sight():
     assert torch.equal(o[0], ref[0]) and bool(o[1].isnan().all())
 
 
+@pytest.mark.parametrize("S,Hq,Hk,hd,page,dtype", [(2, 4, 2, 128, 64, H), (5, 3, 1, 64, 16, BF), (3, 2, 1, 256, 32, H),
+                                                   (8, 4, 1, 128, 16, BF), (6, 8, 1, 128, 64, H), (40, 2, 1, 64, 32, H),
+                                                   (30, 3, 1, 256, 16, BF), (100, 1, 1, 128, 32, H)])
+def test_infinities_between_the_rows_of_a_sequence(S, Hq, Hk, hd, page, dtype):
+    """A V (or K) that is not finite, at a position that only later rows see, reaches those alone."""
+    x = Case([(70, [70 + S, 70 + S + 40, 68 + S]), (0, [S + 3])], S=S, Hq=Hq, Hk=Hk, hd=hd, page=page, dtype=dtype)
+    ref = x.run()
+    for b in range(4):
+        n = int(x.pos[b * S + S - 1]) + 1
+        for back, val in ((1, float("inf")), (S - 1, -float("inf"))):   # seen by the last row; by all but the first
+            y = Case([(70, [70 + S, 70 + S + 40, 68 + S]), (0, [S + 3])], S=S, Hq=Hq, Hk=Hk, hd=hd, page=page, dtype=dtype)
+            p = n - back
+            if b < 3 and p < 70:   # read through the group's owner
+                continue
+            pg, sl = y.table[b, p // page], p % page
+            y.v[pg, 0, sl, 5] = val
+            o = y.run()
+            for r in range(4 * S):
+                sees = r // S == b and int(x.pos[r]) >= p
+                row = o[r].view(Hk, Hq // Hk, hd)
+                if sees:
+                    assert bool((row[0, :, 5] == val).all())
+                    row[0, :, 5] = 0
+                else:
+                    assert torch.equal(o[r], ref[r]) or bool(o[r].isfinite().all())
+            y.v[pg, 0, sl, 5] = 0
+            clean = y.run()
+            clean.view(4 * S, Hk, Hq // Hk, hd)[b * S:(b + 1) * S, 0, :, 5] = 0
+            o.view(4 * S, Hk, Hq // Hk, hd)[b * S:(b + 1) * S, 0, :, 5] = 0
+            torch.testing.assert_close(o.float(), clean.float(), atol=4 * torch.finfo(dtype).eps, rtol=4 * torch.finfo(dtype).eps)
+            y.k[pg, 0, sl] = float("nan")
+            o = y.run()
+            for r in range(4 * S):
+                sees = r // S == b and int(x.pos[r]) >= p
+                assert bool(o[r].view(Hk, Hq // Hk, hd)[0].isnan().all()) == sees
+
+
 def test_bad_entries_are_reported_and_left_out():
     from estudiocanciones_b200 import kernels
     BAD = _lib.HM_ERR_BADINDEX
@@ -277,7 +316,7 @@ def test_bad_entries_are_reported_and_left_out():
         x.plen = torch.tensor([130, 0], dtype=torch.int32, device=DEV)   # that group reads its own pages
         x.owner = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
         x.check(o)
-    for val in ([0, 3, 2], [0, 2, 5], [-1, 2, 4]):
+    for val in ([0, 3, 2], [0, 2, 5], [-1, 2, 4], [-10 ** 9, 2, 4], [10 ** 9, 2, 4], [0, -7, 10 ** 9], [4, 2, 0]):
         x = fresh()
         x.gstart = torch.tensor(val, dtype=torch.int32, device=DEV)
         o = x.run()

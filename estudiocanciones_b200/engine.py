@@ -429,6 +429,7 @@ class HeartMuLaLite:
         self.n_cb = self.shape.n_cb
         self.cb_off = torch.arange(self.n_cb, device=self.dev) * self.vocab
         self.graphs = {}
+        self.prompt_a8 = False  # prompt pass with 8-bit activations (prefill_backbone's a8)
         self._rt = None
         del t
 
@@ -547,7 +548,7 @@ class HeartMuLaLite:
         h[:n_takes, muq_idx] = self.muq_b
         if B == 2 * n_takes:
             h[n_takes:] = self.uncond[0]
-        prefill_backbone(self, h)
+        prefill_backbone(self, h, a8=self.prompt_a8)
         self._rt.pos.fill_(int(text.numel()))
 
     @torch.inference_mode()
@@ -632,7 +633,7 @@ class HeartMuLaLite:
         h[:N, muq_idx] = self.muq_b
         if B == 2 * N:
             h[N:] = self.uncond[0]
-        prefill_backbone(self, h)
+        prefill_backbone(self, h, a8=self.prompt_a8)
         rt.draw_noise = not fixed_noise
         forced = teacher is not None
         if forced:

@@ -36,8 +36,13 @@ def _rows_to_runtime(rt, x_last: torch.Tensor) -> None:
 
 
 @torch.inference_mode()
-def prefill_backbone(model, h: torch.Tensor, keep_f16: bool = True) -> None:
+def prefill_backbone(model, h: torch.Tensor, keep_f16: bool = True, a8: bool = False) -> None:
     """h ``[B, P, D]`` fp16 prompt embeddings on the device.
+
+    a8: the GEMMs take the activations in 8 bits too (``kernels.int8_mm_a8``, a scale per token):
+    twice the tensor-core rate and no fp16 copies of the weights, for results that differ from the
+    default's by the activations' quantisation (at most half a step of 1/127 of a row's largest
+    value).
 
     keep_f16: the GEMMs read fp16 weight tiles (the exact int8 values); with True each
     backbone matrix is converted once and the copy kept for later prompts (2 bytes per
@@ -59,10 +64,12 @@ def prefill_backbone(model, h: torch.Tensor, keep_f16: bool = True) -> None:
     q = torch.empty(M, b0.h * b0.hd, device=dev, dtype=torch.float16)
     # each weight in fp16 (exact int8 values) so the GEMMs read their tiles as they are: kept
     # per matrix, or converted for this prompt into one scratch reused by every matrix
-    wbuf = None if keep_f16 else torch.empty(max(lin.q8.numel() for lin in (b0.qkv, b0.o, b0.w13, b0.w2)),
+    wbuf = None if keep_f16 or a8 else torch.empty(max(lin.q8.numel() for lin in (b0.qkv, b0.o, b0.w13, b0.w2)),
                                              device=dev, dtype=torch.float16)
 
     def gemm(a, lin, **kw):
+        if a8:
+            return kernels.int8_mm_a8(a, lin.q8, lin.s8, **kw)
         if keep_f16:
             if lin.f16 is None:
                 lin.f16 = kernels.dequant_i8(lin.q8)

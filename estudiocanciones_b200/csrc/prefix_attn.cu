@@ -274,7 +274,8 @@ constexpr int kRuns = 8;
 template <int HD>
 struct Smem {
   uint8_t kv[Cfg<HD>::kStages][2][Cfg<HD>::kOperand];
-  float red[4][4][HD];  // four rows of each warp's partial result
+  // four rows of each warp's partial result; for blocks of up to 128 rows 16 columns (64 bytes) of each
+  float red[4][4][HD < 128 ? 128 : HD];
   uint8_t q[Cfg<HD>::kQSmem ? 16 * Cfg<HD>::kQPitch : 16];
   int scan[kMaxJobs + 1];
   int ids[kMaxPre];     // prefix jobs: group and block
@@ -287,6 +288,7 @@ struct Smem {
   int bad[Cfg<HD>::kStages];  // 16-position blocks of the stage without a page
   int abort_flag;
 };
+static_assert(sizeof(Smem<64>::red) >= kBig * 64, "64 bytes of every row of a block");
 static_assert(sizeof(Smem<128>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 128");
 static_assert(sizeof(Smem<64>) + 1024 <= 233472 / 2, "two CTAs per SM at hd 64");
 static_assert(sizeof(Smem<256>) <= 227 * 1024, "shared memory at hd 256");
@@ -882,7 +884,7 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) y[c][j] = q[4 * c];
     }
-    uint4* const buf = reinterpret_cast<uint4*>(&sm.red[0][0][0]) + 128 * warp;  // 2 KB of the 8 (or more)
+    uint4* const buf = reinterpret_cast<uint4*>(&sm.red[0][0][0]) + 128 * warp;  // 2 KB of the 8
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
       __syncwarp();

@@ -191,6 +191,22 @@ def test_crowd():
     assert torch.equal(o, x.run()), "the result does not depend on scheduling"
 
 
+@pytest.mark.parametrize("hd,dtype", [(64, H), (64, BF), (128, H)])
+def test_many_jobs_behind_large_blocks(hd, dtype):
+    """More KV heads and groups of 65 to 128 query rows than the grid has CTAs: each takes several jobs in turn,
+    and its list of them must outlive the blocks before."""
+    x = Case([(1 + g, [2 + g + i for i in range(9 + g % 8)]) for g in range(36)], Hq=128, Hk=16, hd=hd, page=16,
+             dtype=dtype)
+    x.check(x.run(), rows=range(0, x.B, 7))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_several_blocks_a_group_and_head(hd):
+    """Groups of 128 + 40 and 128 + 48 rows a KV head on a prefix of many tiles."""
+    x = Case([(1500, [1501 + 5 * i for i in range(n)]) for n in (21, 21, 22)], Hq=64, Hk=8, hd=hd, page=32)
+    x.check(x.run(), rows=range(0, x.B, 3))
+
+
 def test_groups_are_only_a_way_to_read():
     """With and without groups, and with the groups merged, the outputs agree to rounding."""
     x = Case([(200, [210, 333, 201]), (64, [65, 100])])

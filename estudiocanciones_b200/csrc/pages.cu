@@ -27,6 +27,7 @@ constexpr int kPer = 16;         // reference counts per thread and round
 constexpr int kRound = kMeta * kPer;
 constexpr int kPiece = 4096;     // bytes a warp copies at a time
 constexpr int kCopyThreads = 256;
+constexpr int kMaxPages = 1 << 30;  // rounds over the counts stay inside 32 bits
 
 struct PageState {
   int* table;
@@ -537,7 +538,7 @@ bool bad16(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u);
 
 bool state_ok(const hm_page_state* s) {
   return s && s->table && s->refs && s->n_seqs >= 1 && s->max_pages >= 1 && s->table_ld >= s->max_pages &&
-         s->n_pages >= 1 && s->page >= 1 && s->page <= 1024;
+         s->n_pages >= 1 && s->n_pages <= kMaxPages && s->page >= 1 && s->page <= 1024;
 }
 
 PageState state_of(const hm_page_state* s) {
@@ -545,8 +546,8 @@ PageState state_of(const hm_page_state* s) {
 }
 
 bool pool_ok(const hm_page_pool* p) {
-  return p && !bad16(p->k) && !bad16(p->v) && p->layers >= 1 && p->n_pages >= 1 && p->Hk >= 1 && p->page >= 1 &&
-         p->page <= 1024 && p->row_bytes >= 16 && p->row_bytes % 16 == 0 &&
+  return p && !bad16(p->k) && !bad16(p->v) && p->layers >= 1 && p->n_pages >= 1 && p->n_pages <= kMaxPages &&
+         p->Hk >= 1 && p->page >= 1 && p->page <= 1024 && p->row_bytes >= 16 && p->row_bytes % 16 == 0 &&
          (int64_t)p->page * p->row_bytes <= (1 << 24);
 }
 

@@ -27,7 +27,7 @@ def pool(**kw):
 
 
 BAD_STATES = [dict(table=None), dict(lens=None), dict(refs=None), dict(n_seqs=0), dict(max_pages=0), dict(table_ld=7),
-              dict(n_pages=0), dict(page=0), dict(page=1025)]
+              dict(n_pages=0), dict(n_pages=(1 << 30) + 1), dict(page=0), dict(page=1025)]
 BAD_POOLS = [dict(k=None), dict(v=None), dict(k=24), dict(layers=0), dict(Hk=0), dict(n_pages=15), dict(page=32),
              dict(row_bytes=8), dict(row_bytes=24)]
 
@@ -109,3 +109,29 @@ def test_integer_product(lib):
         assert lib.hm_int8_mm_a8(*{**mm, **kw}.values()) == -1, kw
     assert lib.hm_int8_mm_a8_workspace_bytes(0, 128) == 0
     assert lib.hm_int8_mm_a8_workspace_bytes(65, 128) == 512 + 65 * 128
+
+
+def test_cpu_tensors_are_refused():
+    """There is no CPU path: the Python calls raise before they reach the library."""
+    import torch
+    from estudiocanciones_b200 import kernels as K
+    from estudiocanciones_b200._lib import HMError
+    k = torch.zeros(2, 4, 1, 16, 64, dtype=torch.float16)
+    table, lens, refs = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)
+    ids = torch.zeros(1, dtype=torch.int32)
+    q, pos = torch.zeros(1, 64, dtype=torch.float16), torch.zeros(1, dtype=torch.int64)
+    x, w = torch.zeros(1, 64, dtype=torch.float16), torch.zeros(8, 64, dtype=torch.int8)
+    s = torch.ones(8, dtype=torch.float16)
+    for f in (lambda: K.pages_grow(table, lens, refs, 16, ids), lambda: K.pages_free(table, lens, refs, ids),
+              lambda: K.pages_fork(k, k, table, lens, refs, ids, ids), lambda: K.pages_copy(k, k, ids, ids),
+              lambda: K.pages_compact(k, k, table, refs), lambda: K.prefix_attn(q, k[0], k[0], table, pos),
+              lambda: K.rope_pages(q, torch.zeros(4, 32, 2), pos, q, k[0], k[0], table, 1, 1, 1),
+              lambda: K.quant_tokens(x), lambda: K.int8_mm_a8(x, w, s),
+              lambda: K.gemm_i8a8(w, torch.ones(8), w, s)):
+        with pytest.raises(HMError):
+            f()
+
+
+def test_descriptor_layouts(lib):
+    from estudiocanciones_b200 import _lib
+    assert _lib.abi_mismatches() == []

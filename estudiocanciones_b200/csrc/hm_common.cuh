@@ -114,8 +114,7 @@ HM_DEV bool mbar_wait_ab(uint64_t* bar, uint32_t parity, int* err, volatile int*
   return false;
 }
 
-// mbar_wait_ab for waits that are short and frequent: a few polls before the timer is read
-// (reading globaltimer costs a few hundred nanoseconds, more than such a wait).
+// mbar_wait_ab for waits that are mostly short: up to 64 polls before the timer is read.
 HM_DEV bool mbar_wait_short(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
 #pragma unroll 1
   for (int i = 0; i < 64; ++i)

@@ -1603,6 +1603,7 @@ extern "C" int hm_prefix_attn(const hm_prefix_attn_desc* d, hm_stream_t stream) 
   p.err = d->err;
   // no more CTAs than there can be tiles
   const int64_t most = (s.pre_jobs + (int64_t)s.B * s.own_blocks) * d->Hk * (((int64_t)d->max_pages * pg) / kTile + 1);
+  if (most / ctas > 0x7ffffffe) return HM_EARG;  // a CTA's share is a 32-bit number
   const int grid = static_cast<int>(most < ctas ? most : ctas);
   e = d->hd == 64    ? launch_t<64>(km, vm, p, grid, sms, dev, stream, bf16)
       : d->hd == 128 ? launch_t<128>(km, vm, p, grid, sms, dev, stream, bf16)

@@ -88,9 +88,10 @@ __device__ int block_scan(int v, int* warp_s, int* total) {
 }
 
 // One round over the counts of pages base .. base + kRound - 1: pred(p) for each, their ranks
-// in ascending page order given to use(p, rank) where pred held.  Returns how many held.
+// in ascending page order given to use(p, rank) where pred held.  Returns how many held;
+// use is called for none of them when they are fewer than `least`.
 template <typename Pred, typename Use>
-__device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base, Pred pred, Use use) {
+__device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base, Pred pred, Use use, int least = 0) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   uint32_t mine[kPer];
 #pragma unroll
@@ -126,6 +127,7 @@ __device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base
   }
   __syncthreads();
   const int total = sm.total;
+  if (total < least) return total;
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
     if ((mine[j] >> lane) & 1u) use(base + j * kMeta + tid, sm.cnt[j][w] + __popc(mine[j] & ((1u << lane) - 1u)));
@@ -133,25 +135,26 @@ __device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base
 }
 static_assert(kMeta == 1024, "32 warps: one warp scans kPer counts per lane, and the warps' sums");
 
-// Whether at least `need` pages are free.
-__device__ bool enough_free(MetaSmem& sm, const PageState& P, int need) {
-  int have = 0;
-  for (int base = 0; base < P.n_pages && have < need; base += kRound)
-    have += ranked_round(sm, P.refs, P.n_pages, base, [](int, int r) { return r == 0; }, [](int, int) {});
-  return have >= need;
-}
-
-// give(rank, page) for the `need` lowest free pages (there are enough).
+// give(rank, page) for the `need` lowest free pages, or false (and nothing given) when fewer are free.
+// A pool of one round is read once; a larger one is counted first.
 template <typename Give>
-__device__ void take_free(MetaSmem& sm, const PageState& P, int need, Give give) {
-  int have = 0;
+__device__ bool take_free(MetaSmem& sm, const PageState& P, int need, Give give) {
+  auto is_free = [](int, int r) { return r == 0; };
+  const bool once = P.n_pages <= kRound;
+  int have = once ? need : 0;
+  for (int base = 0; base < P.n_pages && have < need; base += kRound)
+    have += ranked_round(sm, P.refs, P.n_pages, base, is_free, [](int, int) {});
+  if (have < need) return false;
+  have = 0;
   for (int base = 0; base < P.n_pages && have < need; base += kRound) {
     const int h = have;
-    have += ranked_round(sm, P.refs, P.n_pages, base, [](int, int r) { return r == 0; },
+    have += ranked_round(sm, P.refs, P.n_pages, base, is_free,
                          [&](int p, int rank) {
                            if (h + rank < need) give(h + rank, p);
-                         });
+                         },
+                         once ? need : 0);
   }
+  return have >= need;
 }
 
 // The list entry that owns rank r: the last i with off[i] <= r (off ascending, off[n] = total).
@@ -206,20 +209,22 @@ __global__ void __launch_bounds__(kMeta) pages_grow_kernel(PageState P, const in
   __syncthreads();
   if (need) atomicAdd(&sum, static_cast<unsigned long long>(need));
   __syncthreads();
-  if (sum > static_cast<unsigned long long>(P.n_pages) || !enough_free(sm, P, static_cast<int>(sum))) {
+  bool enough = sum <= static_cast<unsigned long long>(P.n_pages);
+  if (enough) {
+    sm.off[tid] = block_scan(need, sm.warp, &sm.off[kMeta]);
+    sm.len[tid] = len;
+    __syncthreads();
+    enough = take_free(sm, P, static_cast<int>(sum), [&](int rank, int p) {
+      const int i = owner_of(sm.off, kMeta, rank);
+      const int col = static_cast<int>((sm.len[i] + P.page - 1) / P.page) + rank - sm.off[i];
+      P.table[sm.a[i] * P.table_ld + col] = p;
+      P.refs[p] = 1;
+    });
+  }
+  if (!enough) {
     if (tid == 0) report_error(P.err, HM_ERR_NOPAGES);
     return;
   }
-  const int total = static_cast<int>(sum);
-  sm.off[tid] = block_scan(need, sm.warp, &sm.off[kMeta]);
-  sm.len[tid] = len;
-  __syncthreads();
-  take_free(sm, P, total, [&](int rank, int p) {
-    const int i = owner_of(sm.off, kMeta, rank);
-    const int col = static_cast<int>((sm.len[i] + P.page - 1) / P.page) + rank - sm.off[i];
-    P.table[sm.a[i] * P.table_ld + col] = p;
-    P.refs[p] = 1;
-  });
   if (s >= 0) P.lens[s] = len + add;
 }
 
@@ -301,17 +306,17 @@ __global__ void __launch_bounds__(kMeta) pages_fork_kernel(PageState P, const in
   sm.off[tid] = block_scan(part > 0, sm.warp, &sm.off[kMeta]);
   __syncthreads();
   const int total = sm.off[kMeta];
-  if (!enough_free(sm, P, total)) {
-    if (tid == 0) report_error(P.err, HM_ERR_NOPAGES);
-    return;
-  }
-  take_free(sm, P, total, [&](int rank, int p) {
+  const bool enough = take_free(sm, P, total, [&](int rank, int p) {
     const int i = owner_of(sm.off, kMeta, rank);
     const int j = static_cast<int>(sm.len[i] / P.page);
     P.table[sm.b[i] * P.table_ld + j] = p;
     P.refs[p] = 1;
     W.moves[rank] = Move{P.table[sm.a[i] * P.table_ld + j], p, static_cast<int>(sm.len[i] % P.page), 0};
   });
+  if (!enough) {
+    if (tid == 0) report_error(P.err, HM_ERR_NOPAGES);
+    return;
+  }
   for (int64_t c = tid; c < cells; c += kMeta) {
     const int i = static_cast<int>(c / P.max_pages), j = static_cast<int>(c % P.max_pages);
     if (sm.b[i] < 0) continue;

@@ -797,33 +797,14 @@ HM_DEV void issue_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, in
   }
 }
 
-// W columns of this thread's TMEM lane (no wait).
-template <int W>
-HM_DEV void tmem_ld_nowait(uint32_t taddr, uint32_t* r);
-template <>
-HM_DEV void tmem_ld_nowait<32>(uint32_t taddr, uint32_t* r) { tmem_ld32_nowait(taddr, r); }
-template <>
-HM_DEV void tmem_ld_nowait<16>(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-template <>
-HM_DEV void tmem_ld_nowait<1>(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(taddr));
-}
-template <>
-HM_DEV void tmem_ld_nowait<8>(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
+// A column of this thread's TMEM lane (no wait).
+HM_DEV void tmem_ld1_nowait(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
 }
 
-// O += P V of this thread's row for positions q0 .. q0 + W - 1 of the tile, those in `sees` only.
+// O += P V of this thread's row for positions q0 .. q0 + 31 of the tile, those in `sees` only.
 // Scores are read back from S.
-template <int HD, typename T, int W>
+template <int HD, typename T>
 __device__ __noinline__ void add_row(const uint8_t* v, int sub_shift, uint32_t tmem, int q0, uint32_t sees, float m,
                                      float scale) {
 #pragma unroll 1
@@ -831,10 +812,10 @@ __device__ __noinline__ void add_row(const uint8_t* v, int sub_shift, uint32_t t
     uint32_t o[32];
     tmem_ld32_nowait(tmem + Cfg<HD>::kTmemO + 32 * c, o);
 #pragma unroll 1
-    for (int p = 0; p < W; ++p) {
+    for (int p = 0; p < kHalf; ++p) {
       uint32_t x;
       __syncwarp();
-      tmem_ld_nowait<1>(tmem + q0 + p, &x);
+      tmem_ld1_nowait(tmem + q0 + p, x);
       tmem_wait_ld();
       if (!((sees >> p) & 1)) continue;
       const float w = ex2(fmaf(__uint_as_float(x), scale, -m));
@@ -857,21 +838,16 @@ __device__ __noinline__ void add_row(const uint8_t* v, int sub_shift, uint32_t t
   }
 }
 
-// Consumers: thread = TMEM lane.  A block of at most 128 / PARTS rows stands PARTS times in the lanes,
-// and copy p does the softmax of columns p * 32 / PARTS .. of every half, its P zero elsewhere: all
-// four warps work (on few rows one warp's exponentials would set the pace), and the copies' O, m
-// and l join at the end.
-template <int HD, typename T, int PARTS, bool kSpread>
+// Consumers: thread = TMEM lane = row of the block.
+template <int HD, typename T, bool kSpread>
 HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, int& ph, int& hph) {
-  constexpr int NW = 4 / PARTS, W = kHalf / PARTS;  // warps per copy, columns of a half per thread
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rg = warp % NW, part = warp / NW, i = 32 * rg + lane;  // row of the block
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = threadIdx.x;  // i: row of the block
   const Job J = run.J;
   const int64_t row_at = run_row(P, run);
   const uint32_t tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16);
-  const bool mine = 32 * rg < J.M;  // whole warps: some rows of this one exist
+  const bool mine = 32 * warp < J.M;  // whole warps: some rows of this one exist
   auto q_row = [&](int k) {         // of row k of this warp's 32 (clamped)
-    const int v = J.i0 + min(32 * rg + k, J.M - 1);
+    const int v = J.i0 + min(32 * warp + k, J.M - 1);
     return reinterpret_cast<const T*>(P.q) + (int64_t)(J.row0 + v / P.G) * P.ld_q + (int64_t)(run.kh * P.G + v % P.G) * HD;
   };
   if (mine) {
@@ -957,23 +933,21 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
       tc_fence_after();
       __syncwarp();
       if (mine) {
-        uint32_t x[W];
-        tmem_ld_nowait<W>(tmem + kHalf * h + W * part, x);
-        // the columns that this row sees, a bit each; then this thread's
+        uint32_t x[kHalf];
+        tmem_ld32_nowait(tmem + kHalf * h, x);
+        // the columns that this row sees, a bit each
         const int from = max(low - a0, 0), to = min(lim - a0, kHalf);
         uint32_t sees = to > from ? (0xffffffffu >> (kHalf - (to - from))) << from : 0u;
         if (bad) sees &= ((bad >> (2 * h)) & 1 ? 0xffff0000u : 0xffffffffu) & ((bad >> (2 * h)) & 2 ? 0xffffu : 0xffffffffu);
-        constexpr uint32_t kAll = 0xffffffffu >> (kHalf - W);
-        sees = (sees >> (W * part)) & kAll;
         tmem_wait_ld();
-        if (__any_sync(0xffffffffu, sees != kAll && sees != 0u)) {
+        if (__any_sync(0xffffffffu, sees != 0xffffffffu && sees != 0u)) {
 #pragma unroll
-          for (int c = 0; c < W; ++c)
+          for (int c = 0; c < kHalf; ++c)
             if (!((sees >> c) & 1)) x[c] = 0xff800000u;  // -infinity
         }
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < W; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(x[c]));
+        for (int c = 0; c < kHalf; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(x[c]));
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * P.scale;
         if (sees == 0u) top = -INFINITY;
         bool grow = false;
@@ -1006,21 +980,19 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
         float sum[2] = {0.f, 0.f};
         uint32_t y[kHalf / 2];
 #pragma unroll
-        for (int c = 0; c < W / 2; ++c) {
+        for (int c = 0; c < kHalf / 2; ++c) {
           const float y0 = ex2(fmaf(__uint_as_float(x[2 * c]), P.scale, -m));
           const float y1 = ex2(fmaf(__uint_as_float(x[2 * c + 1]), P.scale, -m));
           sum[0] += y0;
           sum[1] += y1;
-          const uint32_t z = sees ? Ty<T>::pack(y0, y1) : 0u;
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) y[p * W / 2 + c] = p == part ? z : 0u;
+          y[c] = sees ? Ty<T>::pack(y0, y1) : 0u;
         }
         if (sees) l += sum[0] + sum[1];
         __syncwarp();
         if (kSpread && slow) {
           mbar_wait_short(&sm.o_full[h ^ 1], h ? hph : hph ^ 1, P.err, &sm.abort_flag);  // O at rest, see above
           tc_fence_after();
-          add_row<HD, T, W>(sm.kv[st][1], P.sub_shift, tmem, kHalf * h + W * part, sees, m, P.scale);
+          add_row<HD, T>(sm.kv[st][1], P.sub_shift, tmem, kHalf * h, sees, m, P.scale);
 #pragma unroll
           for (int c = 0; c < kHalf / 2; ++c) y[c] = 0u;
         }
@@ -1047,63 +1019,29 @@ HM_DEV void consume_big(const Params& P, Smem<HD>& sm, const Run& run, int& st, 
   mbar_wait_short(&sm.o_full[1], hph ^ 1, P.err, &sm.abort_flag);
   tc_fence_after();
   if (!seen) m = -INFINITY;
-  // the copies' l for their common maximum
-  if constexpr (PARTS > 1) {
-    sm.mw[warp][lane] = m;
-    sm.lw[warp][lane] = l;
-    named_bar(1, kCons);
-    float top = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) top = fmaxf(top, sm.mw[rg + NW * p][lane]);
-    const float top0 = top == -INFINITY ? 0.f : top;
-    l = 0.f;
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      l += ex2(sm.mw[rg + NW * p][lane] - top0) * sm.lw[rg + NW * p][lane];
-    }
-    m = top;
-  }
-  if (part == 0 && i < J.M) {
+  if (i < J.M) {
     P.pm[row_at + i] = m;
     P.pl[row_at + i] = l;
   }
   // 16 columns at a time through shared memory, where a lane's row becomes four lanes' (whole sectors)
-  // and the copies add up
-  float4* const buf = reinterpret_cast<float4*>(&sm.red[0][0][0]);
-  const int rl = threadIdx.x >> 2, k4 = threadIdx.x & 3;
+  if (mine) {
+    float4* const buf = reinterpret_cast<float4*>(&sm.red[0][0][0]) + 128 * warp;
+    float* const out = P.pa + (row_at + 32 * warp + (lane >> 2)) * HD + 4 * (lane & 3);
 #pragma unroll 1
-  for (int c = 0; c < HD / 16; ++c) {
-    float o[16];
-    __syncwarp();
-    tmem_ld16(tmem + Cfg<HD>::kTmemO + 16 * c, o);
-    if (c) named_bar(1, kCons);  // the last columns have been read
+    for (int c = 0; c < HD / 16; ++c) {
+      float o[16];
+      __syncwarp();  // the last columns have been read
+      tmem_ld16(tmem + Cfg<HD>::kTmemO + 16 * c, o);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      buf[threadIdx.x * 4 + (k ^ ((lane >> 1) & 3))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-    named_bar(1, kCons);
+      for (int k = 0; k < 4; ++k)
+        buf[lane * 4 + (k ^ ((lane >> 1) & 3))] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      __syncwarp();
 #pragma unroll
-    for (int g = 0; g < NW; ++g) {
-      const int row = 32 * g + rl;
-      if (row >= J.M) continue;
-      float4 y = buf[row * 4 + (k4 ^ ((rl >> 1) & 3))];
-      if constexpr (PARTS > 1) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) top = fmaxf(top, sm.mw[g + NW * p][rl]);
-        const float top0 = top == -INFINITY ? 0.f : top;
-        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          const float w = ex2(sm.mw[g + NW * p][rl] - top0);
-          const float4 v = buf[(32 * (g + NW * p) + rl) * 4 + (k4 ^ ((rl >> 1) & 3))];
-          z.x += w * v.x;
-          z.y += w * v.y;
-          z.z += w * v.z;
-          z.w += w * v.w;
-        }
-        y = z;
+      for (int g = 0; g < 4; ++g) {
+        const int row = 8 * g + (lane >> 2);
+        if (32 * warp + row < J.M)
+          *reinterpret_cast<float4*>(out + 8 * g * HD + 16 * c) = buf[row * 4 + ((lane & 3) ^ ((row >> 1) & 3))];
       }
-      *reinterpret_cast<float4*>(P.pa + (row_at + row) * HD + 16 * c + 4 * k4) = y;
     }
   }
   tc_fence_before();
@@ -1291,12 +1229,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
       if (run.tiles == 0) break;
       if (run.J.mt == 16)
         consume<HD, T, kSpread>(P, sm, run, st, ph);
-      else if (run.J.M <= 32)
-        consume_big<HD, T, 4, kSpread>(P, sm, run, st, ph, hph);
-      else if (run.J.M <= 64)
-        consume_big<HD, T, 2, kSpread>(P, sm, run, st, ph, hph);
       else
-        consume_big<HD, T, 1, kSpread>(P, sm, run, st, ph, hph);
+        consume_big<HD, T, kSpread>(P, sm, run, st, ph, hph);
     }
   }
   __syncthreads();

@@ -2,6 +2,7 @@
 
 * :mod:`.kernels` — drop-in counterparts of the reference's ``app/kernels.py``;
 * :mod:`.engine` — ``HeartMuLaLite`` with the reference engine's interface;
+* :mod:`.pages` — a paged KV cache that takes of one prompt share;
 * :mod:`.checkpoint` — the int8 checkpoint format and synthetic weights;
 * :mod:`.shard` — takes sharded over the GPUs of one box.
 

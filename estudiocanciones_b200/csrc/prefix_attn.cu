@@ -28,7 +28,9 @@
 //    256 columns (hd 128) and two CTAs share an SM: one's softmax runs beside the other's products.
 //    O is rescaled only when a row's maximum has grown by more than 2^8 (its reference stays a
 //    little behind: P <= 256, the result does not depend on it), which is rare after a few tiles.
-//    A 64-row tile took 4500 cycles with mma.sync and one warp per 16 rows.
+//    Calls in a graph, us (1 row on 512 positions / 8 rows, two prefixes of 600 / 64 rows on 4096 / 16 rows, two
+//    prefixes of 30001): 10.0 / 14.5 / 42.6 / 68.7; with every block on mma.sync, 16 rows each, 10.0 / 19.7 /
+//    94.2 / 113; with every block on tcgen05 12.7 / 19.5 / 63.2 / 85.6.
 //  * A second small kernel joins the partial results of a row in a fixed order (results do not
 //    depend on scheduling) and writes o; its launch overlaps the first kernel's tail.
 //  * A row that ends inside its group's prefix takes no part in it and reads all its pages itself, so
@@ -37,6 +39,10 @@
 //    that some row sees only in part are looked over, and the products of such a V are added row by
 //    row. Calls with one row per sequence run a variant without that code (kSpread): its registers
 //    and instructions cost a call of 16 sequences on long prefixes 11 % although it never ran.
+//  * What it spends now: the ring alone (no products) takes 22.3 of the 42.6 us and 53.8 of the 68.7 (312 MB: 5.8
+//    TB/s; 4.5 TB/s with the products); a tile of 16 rows costs a CTA ~1500 cycles, one of 24 rows ~2600, one of 128
+//    ~3800, a run of a large block ~9000 more (Q waits behind the ring's loads, the result is 64 KB). Shares
+//    weighted by these costs were slower (49.6 and 77.4 us): they make more such runs.
 // Scores, m, l and a are fp32; the probabilities are rounded to the cache's type for the product
 // with V, as the flat decode attention does (l keeps the unrounded sum).  V rows outside a job's
 // range are zeroed (in registers, in shared memory for tcgen05), so whatever stands there (NaN

@@ -14,6 +14,12 @@ here                   reference                                   C entry point
 ``gemm_i8w``           ``int8_mm`` for M > 16 (``:46-49``)           ``hm_gemm_i8w`` (tcgen05)
 ``prefill_attn``       causal SDPA of ``Block.__call__``            ``hm_prefill_attn``
                        (``app/engine.py:123-153``)
+``rope_pages``         ``rope_cache`` into pages                    ``hm_rope_pages``
+``pages_*``            (none: the static cache has no pages)        ``hm_pages_*``
+``prefix_attn``        (none: ``attn`` reads every row's copy)      ``hm_prefix_attn``
+``int8_mm_a8``         ``int8_mm`` with 8-bit activations           ``hm_int8_mm_a8``
+``quant_tokens``       its two halves                               ``hm_quant_tokens``
+``gemm_i8a8``                                                       ``hm_gemm_i8a8`` (tcgen05)
 ``_rope_cache``        ``_rope_cache[grid](...)`` (``:79-107``)      ``hm_rope_kv_write``
 ``_attn``              ``_attn[grid](...)`` (``:112-153``)           ``hm_decode_attn`` (merged)
 ``_attn_combine``      ``_attn_combine[grid](...)`` (``:157-167``)   nothing (``_attn`` merged)

@@ -286,7 +286,7 @@ struct Smem {
   int scan[kMaxJobs + 1];
   int ids[kMaxPre];     // prefix jobs: group and block
   Run run[kRuns];
-  float mw[4][32], lw[4][32];
+  float mw[4][16], lw[4][16];
   uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages], run_full[kRuns];
   uint64_t s_full[2], o_full[2];  // tcgen05, a half tile: S = Q K^T, O += P V done
   uint64_t q_full, p_full[2];     // Q, P in TMEM (each consumer warp)

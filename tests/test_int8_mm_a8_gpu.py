@@ -95,6 +95,25 @@ def test_tokens_at_every_half(dtype):
         assert torch.equal(sx, (top[:, 0] / 127).float())
 
 
+def test_tokens_of_the_largest_magnitudes():
+    """bf16 rows up to the type's largest value: 127 x leaves the 32-bit range there, the quotients do not."""
+    from estudiocanciones_b200 import kernels
+    halves = torch.arange(-127, 127).double() + 0.5           # 8 significant bits at most: exact in bf16
+    row = torch.cat([halves, torch.tensor([127.0, -127.0]).double()])
+    for e in (113, 114, 117, 118, 120, 121):
+        x = torch.stack([row * 2.0 ** e, row.flip(0) * 2.0 ** (e - 1)]).bfloat16().to(DEV)
+        q, sx = kernels.quant_tokens(x)
+        want, top = rule(x)
+        assert torch.equal(q.double(), want), f"scale 2^{e}"
+        assert torch.equal(sx, (top[:, 0] / 127).float())
+    x = (torch.rand(40, 1040, generator=torch.Generator().manual_seed(5)) * 2 - 1).bfloat16()
+    x[:, 7] = 1.0
+    x = (x.double() * torch.finfo(BF).max).bfloat16().to(DEV)
+    q, sx = kernels.quant_tokens(x)
+    want, top = rule(x)
+    assert torch.equal(q.double(), want) and torch.equal(sx, (top[:, 0] / 127).float())
+
+
 def test_tokens_zero_and_not_finite():
     from estudiocanciones_b200 import kernels
     x = torch.randn(5, 64, device=DEV).half()

@@ -2,7 +2,7 @@
 //
 //   q[m, k] = round(127 x[m, k] / amax[m]),  sx[m] = amax[m] / 127,  amax[m] = max_k |x[m, k]|
 //   acc[m, n] = sum_k q[m, k] * w[n, k]                              (int32, exact: K <= 131072)
-//   STORE: c[m, n] = acc * sx[m] * s[n]  (+ res[m, n])
+//   STORE: c[m, n] = acc * s[n] * sx[m]  (+ res[m, n])
 //   SILU : w = [w1; w3], c[m, f] = silu(a) * b,  a, b = the two halves' scaled sums
 // Everything after the integers is fp32 and rounded once to the activations' type (fp16, bf16).
 // The reference multiplies int8 weights with fp16 activations (app/kernels.py:20-54); with both
@@ -184,8 +184,10 @@ HM_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32
 // silu with the fast exponential and quotient (relative error ~2^-21, rounded to 16 bits next)
 HM_DEV float silu_f(float a) { return __fdividef(a, 1.f + __expf(-a)); }
 
-// 8 consecutive columns of TMEM integers, scaled: v * sx * scl
-HM_DEV float scaled(float bits, float sx, float scl) { return static_cast<float>(__float_as_int(bits)) * sx * scl; }
+// A TMEM integer, scaled.  The channel's scale comes first: an integer times an fp16 value is zero or a normal
+// number, while the token's scale of a bf16 row may be anything that fits 32 bits (times the integer alone it can overflow
+// where the result does not).
+HM_DEV float scaled(float bits, float sx, float scl) { return static_cast<float>(__float_as_int(bits)) * scl * sx; }
 
 // 16 residual values of one row from column `col` on (zero outside)
 template <typename T>

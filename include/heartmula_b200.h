@@ -283,7 +283,7 @@ int hm_dequant_i8_f16(const int8_t* w, void* out, int64_t n, hm_stream_t stream)
  * hm_quant_tokens: sx[m] = max_k |x[m, k]| / 127, q[m, k] = x / sx[m] rounded half to even from the
  *   exact quotient (a zero row: zeros; a row with an infinity or NaN: q = 0, sx = NaN).
  * hm_gemm_i8a8: acc = sum_k q[m, k] * w[n, k] (exact), fp32 from there, one rounding to dtype:
- *   epi HM_EPI_STORE: c[m, n] = acc * sx[m] * s[n] (+ res[m, n]);   c may equal res
+ *   epi HM_EPI_STORE: c[m, n] = acc * s[n] * sx[m] (+ res[m, n]);   c may equal res
  *   epi HM_EPI_SILU : w = [w1; w3] (N = 2F rows), c[m, f] = silu(a) * b  (res must be NULL)
  * hm_int8_mm_a8: both, for x as it comes (ws: hm_int8_mm_a8_workspace_bytes, 16-byte aligned).
  * dtype HM_DT_F16 or HM_DT_BF16 (x, res, c); s fp16 [N]; any M and N >= 1 (rows of 8 columns on

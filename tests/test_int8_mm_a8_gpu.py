@@ -155,6 +155,19 @@ def test_product_with_silu(M, N, K, dtype):
     check(kernels.int8_mm_a8(x, w, s, silu=True), x, w, s, silu=True)
 
 
+@pytest.mark.parametrize("M,N", [(3, 64), (300, 5000)])
+def test_product_of_the_largest_magnitudes(M, N):
+    """bf16 rows near the type's largest value: the integer sum times the token's scale leaves the 32-bit range,
+    the result does not."""
+    from estudiocanciones_b200 import kernels
+    x, w, s = inputs(M, N, 272, BF)
+    x = (x / x.abs().amax(-1, keepdim=True) * 2.0 ** 126).to(BF)
+    s = (s.float() * 2.0 ** -14 / s.float().max()).half()
+    y = kernels.int8_mm_a8(x, w, s)
+    assert bool(y.isfinite().all())
+    check(y, x, w, s)
+
+
 def test_the_longest_sums():
     """K = 131072 with every product at its largest: the sum 127 * 127 * K is held exactly."""
     from estudiocanciones_b200 import kernels

@@ -181,8 +181,15 @@ HM_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32
       : "memory");
 }
 
-// silu with the fast exponential and quotient (relative error ~2^-21, rounded to 16 bits next)
-HM_DEV float silu_f(float a) { return __fdividef(a, 1.f + __expf(-a)); }
+// silu(a) = a c / (c + c e^-a) with the fast exponential and quotient.  c = 2^-8 keeps the divisor below 2^126, above
+// which the fast quotient gives 0, down to a = -92.8, where silu(a) leaves the normal numbers (bf16 has the same); the
+// exponent takes its -8 in the product with log2 e.  The exponential is off by about (2 + |a|) 2^-23, the result is rounded
+// to 16 bits next.
+HM_DEV float silu_f(float a) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(a, -1.4426950408889634f, -8.f)));
+  return __fdividef(a * 0x1p-8f, 0x1p-8f + e);
+}
 
 // A TMEM integer, scaled.  The channel's scale comes first: an integer times an fp16 value is zero or a normal
 // number, while the token's scale of a bf16 row may be anything that fits 32 bits (times the integer alone it can overflow

@@ -168,6 +168,27 @@ def test_product_of_the_largest_magnitudes(M, N):
     check(y, x, w, s)
 
 
+@pytest.mark.parametrize("M,F", [(2, 40), (300, 5000)])
+def test_silu_of_far_negative_values(M, F):
+    """bf16 with a between -91 and -80, where silu(a) still is a normal number and b is large.
+
+    Tolerance, relative: a's conversion, scale and two products move a by 4 half steps, so a e^a by 4 (1 + |a|) of them, b by 4;
+    the exponential is off by 4 + 1.2 |a| steps of 2^-23, the quotient by 2, four products by half a step each; then half a
+    step of the type."""
+    from estudiocanciones_b200 import kernels
+    x = torch.zeros(M, 16, device=DEV, dtype=BF)
+    x[:, 3] = 1.0
+    w = torch.zeros(2 * F, 16, device=DEV, dtype=torch.int8)
+    w[:F, 3], w[F:, 3] = -127, 127
+    s = torch.cat([torch.linspace(80 / 127, 91 / 127, F), torch.full((F,), 60000.0)]).half().to(DEV)
+    y = kernels.int8_mm_a8(x, w, s, silu=True).double()
+    a, b = -127 * s[:F].double(), 127 * s[F:].double()
+    ref = (a * torch.sigmoid(a) * b).expand(M, F)
+    tol = torch.finfo(BF).eps / 2 + (4 * (1 + a.abs()) + 4 + 2 * (4 + 1.2 * a.abs()) + 4 + 4) * 1.01 * 2.0 ** -24
+    d = (y - ref).abs() / ref.abs()
+    assert bool((d <= tol).all()), f"worst {float((d / tol).max()):.3f} of the tolerance"
+
+
 def test_the_longest_sums():
     """K = 131072 with every product at its largest: the sum 127 * 127 * K is held exactly."""
     from estudiocanciones_b200 import kernels

@@ -242,27 +242,29 @@ __global__ void __launch_bounds__(kMeta) pages_free_kernel(PageState P, const in
   if (s >= 0)
     for (int j = 0; j < tid && !bad; ++j) bad = sm.a[j] == s;
   if (any_bad(bad, HM_ERR_BADINDEX, P.err)) return;
+  // The counts go down first: whether the listed rows hold a page more often than it is counted shows only then.
+  // If they do (or name a page that is none), every count goes up again and no row has changed.
   const int64_t cells = (int64_t)n * P.max_pages;
   bad = false;
   for (int64_t c = tid; c < cells; c += kMeta) {
     const int q = sm.a[c / P.max_pages];
     if (q < 0) continue;
     const int p = P.table[q * P.table_ld + c % P.max_pages];
-    if (p >= 0) bad |= p >= P.n_pages || P.refs[p] <= 0;
+    if (p >= 0) bad |= p >= P.n_pages || atomicSub(&P.refs[p], 1) <= 0;
   }
-  if (any_bad(bad, HM_ERR_BADINDEX, P.err)) return;
+  const bool undo = any_bad(bad, HM_ERR_BADINDEX, P.err);
   for (int64_t c = tid; c < cells; c += kMeta) {
     const int q = sm.a[c / P.max_pages];
     if (q < 0) continue;
     int* cell = &P.table[q * P.table_ld + c % P.max_pages];
     const int p = *cell;
     if (p < 0) continue;
-    *cell = -1;
-    if (atomicSub(&P.refs[p], 1) <= 0) {  // held by more rows of the list than its count says
+    if (!undo)
+      *cell = -1;
+    else if (p < P.n_pages)
       atomicAdd(&P.refs[p], 1);
-      report_error(P.err, HM_ERR_BADINDEX);
-    }
   }
+  if (undo) return;
   if (s >= 0) P.lens[s] = 0;
 }
 

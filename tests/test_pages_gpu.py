@@ -184,6 +184,40 @@ def test_disagreeing_tables_are_reported():
     assert kernels.read_errors(DEV) == _lib.HM_ERR_BADINDEX and int(pool.lens[0]) == 20
 
 
+def snapshot(pool):
+    return [t.clone() for t in (pool.k, pool.v, pool.table, pool.lens, pool.refs)]
+
+
+def unchanged(pool, before):
+    return all(torch.equal(a, b) for a, b in zip(snapshot(pool), before))
+
+
+def test_rows_that_hold_more_than_the_counts_say_are_not_freed():
+    """A page counted once that two listed rows, or one row twice, name: the call changes nothing."""
+    from estudiocanciones_b200 import kernels
+    pool, m = make()
+    pool.grow([0, 1, 2], 40)
+    m.grow([0, 1, 2], 40)
+    right = pool.table.clone()
+    pool.table[1, 2] = pool.table[0, 1]
+    before = snapshot(pool)
+    for seqs in ([0, 1], [1, 0], [2, 1, -1, 0]):
+        pool.free(seqs)
+        assert kernels.read_errors(DEV) == _lib.HM_ERR_BADINDEX and unchanged(pool, before)
+    pool.table.copy_(right)
+    pool.table[2, 0] = pool.table[2, 1]
+    before = snapshot(pool)
+    pool.free([0, 2])
+    assert kernels.read_errors(DEV) == _lib.HM_ERR_BADINDEX and unchanged(pool, before)
+    pool.table.copy_(right)
+    pool.fork([0], [3])                              # two full pages that two rows hold, and are counted twice
+    m.fork([0], [3])
+    pool.free([0, 3, 1])
+    m.free([0, 3, 1])
+    assert kernels.read_errors(DEV) == 0
+    m.check(pool)
+
+
 def test_skipped_entries():
     pool, m = make()
     pool.grow([-1, 0, -5, 3], 17)

@@ -92,9 +92,11 @@ __device__ int block_scan(int v, int* warp_s, int* total) {
 
 // One round over the counts of pages base .. base + kRound - 1: pred(p) for each, their ranks
 // in ascending page order given to use(p, rank) where pred held.  Returns how many held;
-// use is called for none of them when they are fewer than `least`.
+// use is called for none of them when they are fewer than `least`.  words (shared memory, if given): a bit
+// for each page of the round, whether it held.
 template <typename Pred, typename Use>
-__device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base, Pred pred, Use use, int least = 0) {
+__device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base, Pred pred, Use use, int least = 0,
+                            uint32_t* words = nullptr) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   uint32_t mine[kPer];
 #pragma unroll
@@ -107,7 +109,10 @@ __device__ int ranked_round(MetaSmem& sm, const int* refs, int n_pages, int base
   __syncthreads();  // sm.cnt and sm.total are free
   if (lane == 0) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sm.cnt[j][w] = __popc(mine[j]);
+    for (int j = 0; j < kPer; ++j) {
+      sm.cnt[j][w] = __popc(mine[j]);
+      if (words) words[j * (kMeta / 32) + w] = mine[j];
+    }
   }
   __syncthreads();
   if (w == 0) {  // exclusive prefix over the (load, warp) order: lane takes 16 consecutive counts
@@ -363,14 +368,52 @@ __global__ void __launch_bounds__(kMeta) pages_copy_list_kernel(const int* __res
 
 // ------------------------------------------------------------------ compact
 // Live pages at or above n_live move into the holes below it, i-th to i-th: the fewest moves,
-// and sources and targets never overlap.
+// and sources and targets never overlap.  The table is looked over first: an entry that names a dead page would
+// end up naming another sequence's.  Then nothing moves, and n_live is the size of the pool, so that the copy kernel
+// renumbers nothing either.
 __global__ void __launch_bounds__(kMeta) pages_compact_kernel(PageState P, MoveList W, int* n_live_out) {
   __shared__ MetaSmem sm;
+  __shared__ uint32_t live_s[kRound / 32];
   const int tid = threadIdx.x;
   pdl_trigger();
+  // The table's cells, kCells of a thread's requested at once, the first ones with the counts: a power of two of
+  // threads to a row (no divisions), row by row.
+  constexpr int kCells = 4;
+  const int lg = P.max_pages <= 32 ? 5 : min(10, 32 - __clz(P.max_pages - 1));
+  int col = tid & ((1 << lg) - 1), row = tid >> lg, cell[kCells];
+  auto fetch = [&] {
+#pragma unroll
+    for (int i = 0; i < kCells; ++i) {
+      cell[i] = col < P.max_pages && row < P.n_seqs ? P.table[row * P.table_ld + col] : -1;
+      row += kMeta >> lg;
+      if (row >= P.n_seqs) {
+        row = tid >> lg;
+        col += 1 << lg;
+      }
+    }
+  };
+  fetch();
   int n_live = 0;
+  const bool once = P.n_pages <= kRound;  // live_s holds the whole pool
   for (int base = 0; base < P.n_pages; base += kRound)
-    n_live += ranked_round(sm, P.refs, P.n_pages, base, [](int, int r) { return r > 0; }, [](int, int) {});
+    n_live += ranked_round(sm, P.refs, P.n_pages, base, [](int, int r) { return r > 0; }, [](int, int) {}, 0, live_s);
+  bool bad = false;
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < kCells; ++i) {
+      const int p = cell[i];
+      if (p >= 0) bad |= p >= P.n_pages || (once ? !((live_s[p >> 5] >> (p & 31)) & 1u) : P.refs[p] <= 0);
+    }
+    if (col >= P.max_pages) break;
+    fetch();
+  }
+  if (any_bad(bad, HM_ERR_BADINDEX, P.err)) {
+    if (tid == 0) {
+      *W.count = 0;
+      *n_live_out = P.n_pages;
+    }
+    return;
+  }
   int holes = 0;
   for (int base = 0; base < n_live; base += kRound) {
     const int h = holes;
@@ -382,7 +425,6 @@ __global__ void __launch_bounds__(kMeta) pages_compact_kernel(PageState P, MoveL
     const int h = movers;
     movers += ranked_round(sm, P.refs, P.n_pages, base,
                            [&](int p, int r) {
-                             if (p >= n_live) W.map[p] = -1;
                              return p >= n_live && r > 0;
                            },
                            [&](int p, int rank) {
@@ -450,11 +492,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_c
       int* cell = &C.P.table[c / C.P.max_pages * C.P.table_ld + c % C.P.max_pages];
       const int p = *cell;
       if (p < n_live) continue;
-      const int to = p < C.P.n_pages ? C.W.map[p] : -1;
-      if (to >= 0)
-        *cell = to;
-      else
-        report_error(C.P.err, HM_ERR_BADINDEX);  // the entry names a page that nobody holds
+      if (p < C.P.n_pages) *cell = C.W.map[p];  // (not so only in a table that was refused)
     }
   }
 }

@@ -424,7 +424,7 @@ def pages_copy(k, v, src, dst) -> None:
 def pages_compact(k, v, table, refs) -> torch.Tensor:
     """Pack the live pages (``refs > 0``) into the lowest numbers: those at or above their count
     move into the free ones below it, in ascending order, and the table follows.  Returns the
-    count, int32 ``[1]`` on the device."""
+    count, int32 ``[1]`` on the device (the pool's size when the call is refused)."""
     _device_of("pages_compact", table, k, v)
     pool, n_pages, page = _page_pool("pages_compact", k, v)
     idx, st = _page_state("pages_compact", table, None, refs, page)

@@ -349,7 +349,8 @@ int hm_pages_fork(const hm_page_state* s, const hm_page_pool* pool, const int* s
 int hm_pages_copy(const hm_page_pool* pool, const int* src, const int* dst, int n, void* ws, size_t ws_bytes, int* err,
                   hm_stream_t stream);
 /* Live pages at or above *n_live (their number, written) move into the free ones below it, i-th
- * to i-th in ascending order, and the table follows: afterwards pages [0, *n_live) are live. */
+ * to i-th in ascending order, and the table follows: afterwards pages [0, *n_live) are live.  A call
+ * that is refused (an entry of the table names a page that nobody holds, or none) writes n_pages there. */
 int hm_pages_compact(const hm_page_state* s, const hm_page_pool* pool, int* n_live, void* ws, size_t ws_bytes,
                      hm_stream_t stream);
 

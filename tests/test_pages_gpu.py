@@ -218,6 +218,26 @@ def test_rows_that_hold_more_than_the_counts_say_are_not_freed():
     m.check(pool)
 
 
+@pytest.mark.parametrize("stale", [2, 7, 20, 40, 1000])
+def test_compaction_checks_the_table_first(stale):
+    """An entry that names a page nobody holds (below the live count, above it) or none of the pool's: nothing
+    changes, and the count returned is the pool's size, below which every live page lies."""
+    from estudiocanciones_b200 import kernels
+    pool, m = make()
+    pool.grow([0, 1, 2, 3], 32)
+    pool.free([1, 3])                                # live 0 1 4 5 -> 0 1 2 3; 2 3 6 7 and up are free
+    m.grow([0, 1, 2, 3], 32)
+    m.free([1, 3])
+    pool.table[9, 5] = stale
+    before = snapshot(pool)
+    n = pool.compact()
+    assert kernels.read_errors(DEV) == _lib.HM_ERR_BADINDEX and unchanged(pool, before) and int(n) == 40
+    pool.table[9, 5] = -1
+    assert int(pool.compact()) == m.compact() == 4
+    assert kernels.read_errors(DEV) == 0
+    m.check(pool)
+
+
 def test_skipped_entries():
     pool, m = make()
     pool.grow([-1, 0, -5, 3], 17)

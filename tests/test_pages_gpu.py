@@ -277,6 +277,50 @@ def test_long_lists_and_a_wide_pool():
     assert torch.equal(pool.table.cpu()[seqs.long(), :7], to[want].int())
 
 
+def test_compaction_of_a_wide_pool_moves_the_bytes():
+    """Several rounds of counts; every moved page's K and V stand behind its new number, the others stay."""
+    from estudiocanciones_b200.pages import PagePool
+    n = 40000
+    pool = PagePool(2, n, 2, 8, 900, 40, 2, torch.float16, DEV)
+    g = torch.Generator().manual_seed(4)
+    for t in (pool.k, pool.v):
+        t.copy_(torch.randn(t.shape, generator=g))
+    live = torch.randperm(n, generator=g)[:900 * 20].view(900, 20)
+    pool.table.copy_(live)
+    pool.refs[live.flatten().to(DEV)] = 1
+    old_k, old_v, at = pool.k[:, live.flatten()], pool.v[:, live.flatten()], live.flatten()
+    assert int(pool.compact()) == 18000
+    new = pool.table.flatten().long()
+    assert torch.equal(new.sort().values.cpu(), torch.arange(18000)) and int((new.cpu() != at).sum()) == int((at >= 18000).sum())
+    assert torch.equal(pool.k[:, new], old_k) and torch.equal(pool.v[:, new], old_v)
+
+
+@pytest.mark.parametrize("n_seqs,max_pages,n_pages", [(1, 1, 4), (1, 5000, 64), (70, 33, 300), (5, 1500, 20000), (1100, 20, 64),
+                                                      (3, 1025, 64), (33, 32, 16385)])
+def test_compaction_looks_at_every_cell(n_seqs, max_pages, n_pages):
+    """One stale entry anywhere in tables of all shapes, in pools of one and of several rounds, is found."""
+    from estudiocanciones_b200 import kernels
+    from estudiocanciones_b200.pages import PagePool
+    rng = random.Random(n_seqs + max_pages)
+    pool = PagePool(1, n_pages, 1, 8, n_seqs, max_pages, 1, torch.float16, DEV)
+    pool.refs[n_pages // 2:] = 1
+    pool.table.copy_(torch.randint(n_pages // 2, n_pages, pool.table.shape, dtype=torch.int32))
+    before = snapshot(pool)
+    ends = [(0, 0), (n_seqs - 1, max_pages - 1), (0, max_pages - 1), (n_seqs - 1, 0)]
+    for at in ends + [(rng.randrange(n_seqs), rng.randrange(max_pages)) for _ in range(20)]:
+        right = int(pool.table[at])
+        pool.table[at] = rng.choice([rng.randrange(n_pages // 2), n_pages, n_pages + 7])
+        n = pool.compact()
+        assert kernels.read_errors(DEV) == _lib.HM_ERR_BADINDEX and int(n) == n_pages
+        pool.table[at] = right
+        assert unchanged(pool, before)
+    n = n_pages - n_pages // 2
+    assert int(pool.compact()) == n and kernels.read_errors(DEV) == 0
+    old, hole = before[2].long(), torch.arange(n_pages // 2, device=DEV)   # page i of the upper half above n goes to hole i
+    moved = torch.where(old >= n, hole[(old - n).clamp(0, len(hole) - 1)], old)
+    assert torch.equal(pool.table.long(), moved)
+
+
 def test_captured_calls_replay():
     """grow + fork + free in one graph: every replay does the work on the state it finds."""
     from estudiocanciones_b200._lib import capture_graph

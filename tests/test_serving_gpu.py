@@ -143,6 +143,52 @@ def test_takes_of_two_prompts(P, page):
     assert pool.free_pages() == 64 and bool((pool.table == -1).all())
 
 
+def test_takes_go_on_after_their_pages_move():
+    """A sequence in front of the takes ends in the middle of the song and its room is closed: the captured frame
+    gives bit for bit what it gives in a pool where nothing moves."""
+    from estudiocanciones_b200._lib import capture_graph
+    from estudiocanciones_b200.pages import PagePool
+    net = Net()
+    P, page, frames, L = 70, 16, 14, 512
+    g = torch.Generator().manual_seed(11)
+    prompts = torch.randn(2 * P, net.D, generator=g).half().to(DEV)
+    steps = torch.randn(frames, 4, net.D, generator=g).half().to(DEV)
+    two = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    takes = torch.tensor([2, 3, 4, 5], dtype=torch.int32, device=DEV)
+    groups = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 2, 4], [0, 1], [P, P])]
+
+    def song(moves):
+        pool = PagePool(len(net.layers), 64, net.Hk, net.hd, 10, L, page, torch.float16, DEV)
+        pool.grow([8], 100)                                  # in front of everything
+        pool.grow([0, 1], P)
+        net.run(prompts, paged(net, pool, torch.arange(P, device=DEV).repeat(2), P, two, ()))
+        pool.fork(two.repeat_interleave(2), takes)
+        pos = torch.full((4,), P - 1, device=DEV)
+        xin = torch.zeros(4, net.D, device=DEV).half()
+
+        def frame():
+            pos.add_(1)
+            pool.grow(takes, 1)
+            return net.run(xin, paged(net, pool, pos, 1, takes, groups))
+        gr, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with capture_graph(gr, st):
+            y = frame()
+        out = []
+        for f in range(frames):
+            if f == 4 and moves:
+                before, used = pool.table.clone(), pool.k.shape[1] - pool.free_pages()
+                pool.free([8])
+                assert int(pool.compact()) == used - 7
+                assert int((pool.table[:6] != before[:6]).sum()) > 0
+            xin.copy_(steps[f])
+            gr.replay()
+            out.append(y.clone())
+        del gr
+        return torch.stack(out)
+    assert torch.equal(song(True), song(False))
+
+
 def test_prompt_pass_with_8_bit_activations():
     """prefill_backbone(a8=True) is the layer loop written out with int8_mm_a8, and makes no fp16 copies."""
     from estudiocanciones_b200 import kernels as K

@@ -25,7 +25,10 @@ class PagePool:
     """K and V pages of every layer and the bookkeeping of the sequences that hold them.
 
     ``k``, ``v`` ``[layers, n_pages, kv_heads, page, hd]``; ``table [max_seqs, max_pages]`` int32
-    (-1 = none); ``lens [max_seqs]`` int64; ``refs [n_pages]`` int32 (0 = free)."""
+    (-1 = none); ``lens [max_seqs]`` int64; ``refs [n_pages]`` int32 (0 = free).
+
+    The page calls and ``rope_pages`` take any ``page`` up to 1024 and any ``hd`` that is a multiple of 8;
+    ``prefix_attn`` reads pages of 16, 32 or a multiple of 64 positions with ``hd`` 64, 128 or 256."""
 
     def __init__(self, layers: int, n_pages: int, kv_heads: int, hd: int, max_seqs: int, max_len: int, page: int = 64,
                  dtype: torch.dtype = torch.float16, device="cuda"):
@@ -33,6 +36,8 @@ class PagePool:
             raise HMError("PagePool: every size is at least 1")
         if dtype not in (torch.float16, torch.bfloat16):
             raise HMError("PagePool: fp16 or bf16")
+        if page > 1024 or hd % 8:
+            raise HMError("PagePool: pages of at most 1024 positions, hd a multiple of 8")
         shape = (layers, n_pages, kv_heads, page, hd)
         self.page = page
         self.k = torch.zeros(shape, dtype=dtype, device=device)

@@ -132,6 +132,18 @@ def test_cpu_tensors_are_refused():
             f()
 
 
+def test_pool_sizes_that_no_call_takes():
+    """Refused when the pool is made, not at the first call."""
+    import torch
+    from estudiocanciones_b200._lib import HMError
+    from estudiocanciones_b200.pages import PagePool
+    PagePool(1, 2, 1, 8, 1, 1024, 1024, torch.float16, "cpu")
+    for kw in (dict(page=1025), dict(hd=4), dict(hd=12), dict(hd=100), dict(page=0), dict(n_pages=0), dict(dtype=torch.float32)):
+        a = dict(layers=1, n_pages=2, kv_heads=1, hd=64, max_seqs=1, max_len=64, page=16, dtype=torch.float16)
+        with pytest.raises(HMError):
+            PagePool(**{**a, **kw}, device="cpu")
+
+
 def test_descriptor_layouts(lib):
     from estudiocanciones_b200 import _lib
     assert _lib.abi_mismatches() == []

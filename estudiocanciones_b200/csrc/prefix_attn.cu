@@ -1060,8 +1060,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
                        const __grid_constant__ Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(smem_raw);
-  if (smem_u32(smem_raw) & 1023u) {  // (the same for every CTA: all return)
+  if (smem_u32(smem_raw) & 1023u) {  // (the same for every CTA: all return, and the join finds jobs without tiles)
     if (threadIdx.x == 0) report_error(P.err, HM_ERR_TIMEOUT);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i < kPlanInts; i += kThreads) P.plan[i] = i == 0;
     return;
   }
   constexpr int NST = Cfg<HD>::kStages;

@@ -263,7 +263,10 @@ __global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------ TMA producers
     // the weights do not depend on the launch before, so only the tokens wait for it
-    if (warp == 2) pdl_wait();
+    if (warp == 2) {
+      pdl_wait();
+      fence_proxy_async_global();  // the launch before wrote the tokens; TMA reads them
+    }
     for (int kb = 0, s = 0, ph = 1; kb < nk; ++kb) {
       if (kb >= nst && !mbar_wait_short(&sm.empty[s], ph, err, abort_s)) break;
       if (elect_one()) {
@@ -501,6 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       prefetch_tensormap(&amap);
       prefetch_tensormap(&wmap);
     }
+    fence_proxy_async_global();  // the launch before wrote the tokens; TMA reads them
     __syncwarp();
     const uint32_t full0 = dsmem_addr(&sm.full[0], 0);
     int g = 0;

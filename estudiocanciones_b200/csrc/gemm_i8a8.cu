@@ -19,7 +19,7 @@
 // 128 bytes) with the int32 sums in TMEM:
 //  * gemm_small: one MT x BN tile per CTA, MT = 64 or 128, BN = 32 .. 128.  For few tokens the weights are all the
 //    traffic, so BN is chosen to put the weight stream on as many SMs as there are, and a CTA
-//    keeps a ring of up to ~100 KB in flight.  Only the rows that exist are loaded: the MMA's
+//    keeps a ring of up to 200 KB in flight (106 KB where two CTAs share an SM).  Only the rows that exist are loaded: the MMA's
 //    other rows read whatever lies behind them in shared memory, and nobody reads their sums.
 //    In hm_int8_mm_a8 the weight stream starts before the quantisation has finished
 //    (programmatic dependent launch; the weights do not depend on it).
@@ -614,7 +614,7 @@ cudaError_t max_smem(K kernel, std::atomic<bool>* configured, int dev, size_t by
 }
 
 // A small CTA's ring: two CTAs per SM, or one when the grid has no more CTAs than SMs (8 x 5120 x 4096:
-// 7.1 us with 200 KB, 9.0 with 106; 64 x 16384 x 4096: 11.7, 14.6).
+// 7.2 us with 200 KB, 9.2 with 106; 64 x 16384 x 4096: 11.4, 13.9).
 constexpr int kRingTwo = 106 * 1024, kRingOne = 200 * 1024;
 
 template <int BN, int EPI, int MT, typename T>
@@ -659,6 +659,8 @@ cudaError_t launch_pair(const CUtensorMap& am, const CUtensorMap& wm, GemmParams
   if (e != cudaSuccess) return e;
   constexpr int WT = EPI == HM_EPI_SILU ? BN2 / 2 : BN2;
   p.ntiles = (p.N + WT - 1) / WT;
+  // the tiles in flight share the larger operand's rows: 16384 x 4096 x 4096 in 170 us with N fast, 187 with M fast;
+  // 4096 x 16384 x 4096 191 and 185; 8192 x 2048 x 4096 48.2 and 47.1 (both fit the L2)
   p.n_fast = p.M > (EPI == HM_EPI_SILU ? 2 * p.N : p.N);
   const int64_t tiles = (int64_t)((p.M + 2 * BM - 1) / (2 * BM)) * p.ntiles;
   const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
@@ -672,8 +674,8 @@ cudaError_t launch_gemm(const int8_t* q, int64_t ldq, const int8_t* w, GemmParam
   if (e != cudaSuccess) return e;
   CUtensorMap am, wm;
   const int64_t pair_tiles = (int64_t)((p.M + 255) / 256) * ((wrows + 255) / 256);
-  // pairs once half of them have a tile; at K = N = 4096, us small / pairs: M 256 10.7 / 15.4, 512 12.6 / 15.7,
-  // 640 17.5 / 16.2, 1024 20.3 / 16.5, 2048 36.1 / 26.2
+  // pairs once half of them have a tile; at K = N = 4096, us small / pairs: M 256 10.6 / 15.4, 512 12.6 / 15.8,
+  // 640 17.8 / 16.1, 1024 18.3 / 16.5, 2048 34.0 / 25.9
   if (p.M > BM && pair_tiles >= sms / 4) {
     if (!tile_map(q, p.M, p.K, ldq, BM, &am) || !tile_map(w, wrows, p.K, p.K, BM, &wm)) return cudaErrorInvalidValue;
     return launch_pair<EPI, T>(am, wm, p, sms, dev, pdl, st);
@@ -681,7 +683,9 @@ cudaError_t launch_gemm(const int8_t* q, int64_t ldq, const int8_t* w, GemmParam
   const int mt = (p.M + BM - 1) / BM;
   p.m_box = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
   // the tile width whose CTAs cost an SM the least: cycles per MMA (measured, with a share of the
-  // waits) times the CTAs that an SM gets.  1 x 5120 x 4096: 8.2 us at 64, 8.9 at 32, 10.1 at 128.
+  // waits) times the CTAs that an SM gets.  us at 32 / 64 / 128, K 4096, the rule's in brackets: 1 x 1024 [6.1] / 6.9 / 10.6,
+  // 1 x 5120 8.1 / [7.2] / 10.7, 8 x 16384 14.2 / 11.1 / [11.4], 64 x 5120 9.3 / [7.6] / 11.1, 64 x 16384 17.8 / 11.0 / [11.8],
+  // 128 x 5120 14.5 / [11.0] / 12.7, 128 x 16384 26.6 / 16.9 / [12.7], 333 x 4096 (K 2048) 15.2 / 10.5 / [8.3].
   const int64_t cycles[2][3] = {{37, 45, 77}, {53, 61, 77}};
   int bn = 0;
   int64_t best = INT64_MAX;

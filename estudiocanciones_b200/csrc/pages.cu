@@ -11,11 +11,12 @@
 // lowest number first, in the order of the list, so the result does not depend on scheduling.
 // The r-th free page is found by ballots: 16 coalesced loads per thread, 16 x 32 warp counts
 // scanned by one warp; a pool of 16384 pages is one round.  Bound by its chain of memory latencies and
-// barriers: grow and free take 2.5 us in a graph, the list of a fork or a compaction 5 to 8.
+// barriers: grow and free take 2.5 to 2.8 us in a graph, the list of a fork 5 to 8, that of a compaction 8 to 10 (it looks
+// at the whole table too: 64 sequences of 512 pages cost it 6 more).
 // Data (copy kernel, every SM): pure HBM traffic, 2 bytes moved per byte kept.  A warp takes a
 // piece of 4 KB (8 x 16 bytes per lane in flight) of one (page, layer, K or V, head).  Only the
 // rows that hold positions are copied.  Compacting 128 pages of 4 MB, half of them free (32 pages move, 268 MB
-// read and written), takes 55 us with its list and two small copies that restore the table and the counts
+// read and written), takes 58 us with its list and two small copies that restore the table and the counts
 // for the next pass (4.9 TB/s); eight forks of 600 positions in 28 layers 17 us.
 // The copy kernel reads the list that the bookkeeping kernel wrote, so nothing returns to the
 // host and both can be captured.

@@ -29,8 +29,9 @@
 //    O is rescaled only when a row's maximum has grown by more than 2^8 (its reference stays a
 //    little behind: P <= 256, the result does not depend on it), which is rare after a few tiles.
 //    Calls in a graph, us (1 row on 512 positions / 8 rows, two prefixes of 600 / 64 rows on 4096 / 16 rows, two
-//    prefixes of 30001): 10.0 / 14.5 / 42.6 / 68.7; with every block on mma.sync, 16 rows each, 10.0 / 19.7 /
-//    94.2 / 113; with every block on tcgen05 12.7 / 19.5 / 63.2 / 85.6.
+//    prefixes of 30001): 10.0 / 14.5 / 42.6 / 68.9; with every block on mma.sync, 16 rows each, 10.0 / 19.6 /
+//    91.5 / 108; with every block on tcgen05 12.4 / 18.6 / 58.1 / 78.8.  Several rows a sequence: 8 x 8 rows behind a prefix of
+//    600 26.9, two prompts of 512 65, one of 1024 84.
 //  * A second small kernel joins the partial results of a row in a fixed order (results do not
 //    depend on scheduling) and writes o; its launch overlaps the first kernel's tail.
 //  * A row that ends inside its group's prefix takes no part in it and reads all its pages itself, so
@@ -1257,8 +1258,8 @@ HM_DEV int quotient(int64_t x, int d) {
 // prefix's, every WPR-th by one warp.  Nothing to join (a padding row): zeros.  The kernel is a chain
 // of memory latencies, so everything that can be is requested at once: the job list's entries, then
 // the maxima, sums and first columns together.  Four warps a pair while all pairs fit the SMs at once
-// (16 x 24 pairs of ~17 splits: 71.8 us a call, 76.5 with one warp each), one where there are more
-// (64 x 32 pairs of ~8 splits: 45.3 us, 48.7 with four).
+// (16 x 24 pairs of ~17 splits: 69.1 us a call, 72.9 with one warp each), one where there are more
+// (64 x 32 pairs of ~8 splits: 42.4 us, 45.5 with four).
 template <int HD, typename T, int WPR>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params P) {
   __shared__ float part_s[WPR == 1 ? 1 : 4][HD];

@@ -39,10 +39,11 @@ def _rows_to_runtime(rt, x_last: torch.Tensor) -> None:
 def prefill_backbone(model, h: torch.Tensor, keep_f16: bool = True, a8: bool = False) -> None:
     """h ``[B, P, D]`` fp16 prompt embeddings on the device.
 
-    a8: the GEMMs take the activations in 8 bits too (``kernels.int8_mm_a8``, a scale per token):
-    twice the tensor-core rate and no fp16 copies of the weights, for results that differ from the
-    default's by the activations' quantisation (at most half a step of 1/127 of a row's largest
-    value).
+    a8: the GEMMs take the activations in 8 bits too (``kernels.int8_mm_a8``, a scale per token): no fp16
+    copies of the weights and 25.3 ms instead of 41.5 for 8 x 1024 tokens at the 3B shape, for results that
+    differ from the default's by the activations' quantisation (at most half a step of 1/127 of a row's
+    largest value in every product): with random weights the last position's logits move by 0.08 to 0.11 of
+    their norm over the 28 layers.
 
     keep_f16: the GEMMs read fp16 weight tiles (the exact int8 values); with True each
     backbone matrix is converted once and the copy kept for later prompts (2 bytes per

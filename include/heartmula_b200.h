@@ -282,7 +282,8 @@ int hm_dequant_i8_f16(const int8_t* w, void* out, int64_t n, hm_stream_t stream)
  * (app/kernels.py:40-54) with the activations in 8 bits too.
  * hm_quant_tokens: sx[m] = max_k |x[m, k]| / 127, q[m, k] = x / sx[m] rounded half to even from the
  *   exact quotient (a zero row: zeros; a row with an infinity or NaN: q = 0, sx = NaN).
- * hm_gemm_i8a8: acc = sum_k q[m, k] * w[n, k] (exact), fp32 from there, one rounding to dtype:
+ * hm_gemm_i8a8: acc = sum_k q[m, k] * w[n, k] (exact for |q| <= 127, as hm_quant_tokens writes them; any w), fp32 from
+ *   there, one rounding to dtype:
  *   epi HM_EPI_STORE: c[m, n] = acc * s[n] * sx[m] (+ res[m, n]);   c may equal res
  *   epi HM_EPI_SILU : w = [w1; w3] (N = 2F rows), c[m, f] = silu(a) * b  (res must be NULL)
  * hm_int8_mm_a8: both, for x as it comes (ws: hm_int8_mm_a8_workspace_bytes, 16-byte aligned).
@@ -315,7 +316,8 @@ int hm_prefill_attn(const void* q, const void* kc, const void* vc, void* o, int 
  * and changes nothing (HM_ERR_BADINDEX: a bad or repeated entry, or a table that disagrees
  * with refs; HM_ERR_NOPAGES: too few free pages).  Free pages are handed out lowest number
  * first, in the order of the list.  Lists hold 1 to 1024 int32 entries; a negative entry (of
- * dst, for a pair) is skipped.  Calls on one state must not overlap on the GPU. */
+ * dst, for a pair) is skipped.  Calls on one state must not overlap on the GPU.  Cells behind a sequence's
+ * lens are -1 (the calls keep them so, and write there without looking). */
 typedef struct {
   int* table;
   int64_t table_ld;
@@ -358,7 +360,8 @@ int hm_pages_compact(const hm_page_state* s, const hm_page_pool* pool, int* n_li
  * [R, (Hq+2Hk)*hd] (row pitch ld_qkv) belongs to table row seqs[r / S] (seqs NULL: r / S) at
  * position pos[r]; q_out [R, Hq*hd] (pitch ld_q), k / v one layer's pool [n_pages, Hk, page, hd].
  * dtype HM_DT_F16 or HM_DT_BF16 (qkv, q_out, k, v).  pos[r] < 0: a padding row, q_out zero and
- * nothing written; a position without a page: the same, with HM_ERR_BADINDEX. */
+ * nothing written; a position without a page: the same, with HM_ERR_BADINDEX.  Two rows on one position of one
+ * page leave a mixture of both there. */
 int hm_rope_pages(const void* qkv, int64_t ld_qkv, const float* rope, int rope_rows, const int64_t* pos, void* q_out,
                   int64_t ld_q, void* k, void* v, int dtype, const int* table, int64_t table_ld, const int* seqs,
                   int n_table, int max_pages, int n_pages, int page, int R, int S, int Hq, int Hk, int hd, int* err,

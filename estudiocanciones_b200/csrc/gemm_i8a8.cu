@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kSmallThreads) gemm_small_kernel(const __grid_
       }
     }
   }
+  settle(abort_s);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -571,6 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       });
     }
   }
+  settle(abort_s);
   tc_fence_before();
   cluster_sync_all();  // neither CTA leaves while the pair's copies, MMAs or commits may touch its memory
   if (warp == 1) {

@@ -122,6 +122,16 @@ HM_DEV bool mbar_wait_short(uint64_t* bar, uint32_t parity, int* err, volatile i
   return mbar_wait_ab(bar, parity, err, abort_flag);
 }
 
+// After a wait gave up, copies and matrix products that were issued may still be on their way, and a CTA must
+// not hand its memory back before they land.  They take microseconds: each thread that sees the flag stays a millisecond
+// (at most 2^20 looks at the clock) before the CTA's last barrier.
+HM_DEV void settle(const volatile int* abort_flag) {
+  if (!*abort_flag) return;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 0; i < (1u << 20) && globaltimer_ns() - t0 < 1000000ull; ++i) {
+  }
+}
+
 // ---------------------------------------------------------------- thread-block clusters
 HM_DEV uint32_t cluster_ctarank() {
   uint32_t r;

@@ -1242,6 +1242,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas)
         consume_big<HD, T, kSpread>(P, sm, run, st, ph, hph);
     }
   }
+  settle(&sm.abort_flag);
   __syncthreads();
   if (P.big && tid >= kThreads - 32) {
     tc_fence_after();

@@ -182,7 +182,7 @@ HM_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32
 }
 
 // silu(a) = a c / (c + c e^-a) with the fast exponential and quotient.  c = 2^-8 keeps the divisor below 2^126, above
-// which the fast quotient gives 0, down to a = -92.8, where silu(a) leaves the normal numbers (bf16 has the same); the
+// which the fast quotient gives 0, down to a = -92.8; silu(a) leaves the normal numbers (bf16 has the same) at -91.9.  The
 // exponent takes its -8 in the product with log2 e.  The exponential is off by about (2 + |a|) 2^-23, the result is rounded
 // to 16 bits next.
 HM_DEV float silu_f(float a) {
